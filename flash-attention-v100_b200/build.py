@@ -11,7 +11,9 @@ architecture, no third-party headers.  nvcc cross-compiles without a GPU.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -26,7 +28,7 @@ EXT_PATH = os.path.join(HERE, EXT_NAME + (sysconfig.get_config_var("EXT_SUFFIX")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -35,6 +37,17 @@ def _newer(target: str, sources) -> bool:
         return False
     t = os.path.getmtime(target)
     return all(os.path.getmtime(s) <= t for s in sources)
+
+
+def _with_includes(source: str, seen=None):
+    """A source file and what it includes in quotes, directly or not."""
+    seen = [] if seen is None else seen
+    if source not in seen:
+        seen.append(source)
+        with open(source) as f:
+            for name in re.findall(r'^#include "([^"]+)"', f.read(), flags=re.M):
+                _with_includes(os.path.normpath(os.path.join(os.path.dirname(source), name)), seen)
+    return seen
 
 
 def _run(cmd):
@@ -53,9 +66,14 @@ def build_library(force: bool = False, verbose_ptxas: bool = False) -> str:
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
     nvcc = os.path.join(_cuda_home(), "bin", "nvcc")
-    cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose_ptxas else [])
-    cmd += ["-o", LIB_PATH, os.path.join(CSRC, "fmha_api.cu")]
-    _run(cmd)
+    # every .cu file on its own, side by side: the kernels are many, and none needs another's file
+    units = [s for s in sources if s.endswith(".cu")]
+    objects = [os.path.join(LIB_DIR, os.path.basename(s)[:-3] + ".o") for s in units]
+    cmds = [[nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose_ptxas else []) + ["-c", "-o", o, s]
+            for s, o in zip(units, objects) if force or not _newer(o, _with_includes(s))]
+    with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, os.cpu_count() or 1)) as pool:
+        list(pool.map(_run, cmds))
+    _run([nvcc] + NVCC_FLAGS + ["-shared", "-o", LIB_PATH] + objects)
     return LIB_PATH
 
 

@@ -373,6 +373,228 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
                               causal, seqused_q, seqused_k));
 }
 
+// ---------------------------------------------------------------------------------------------
+// The paged key/value cache: what new tokens' K and V are written to and read back from, and the
+// attention over it.  No counterpart in the reference.
+// ---------------------------------------------------------------------------------------------
+int32_t int32_of(int64_t n, const char* what) {
+  TORCH_CHECK(n <= INT32_MAX, what, " is too large: ", n);
+  return static_cast<int32_t>(n);
+}
+
+// the pools, scales and block table of a cache for tensors of `type` and (batch, heads, D) on `device`
+FmhaPagedCache cache_of(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+                        const OptTensor& k_scale, const OptTensor& v_scale, at::ScalarType type, c10::Device device,
+                        int64_t batch, int64_t heads, int64_t head_dim) {
+  FmhaPagedCache c = {};
+  const bool e4m3 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
+  for (const at::Tensor* t : {&k_cache, &v_cache}) {
+    TORCH_CHECK(t->is_cuda() && t->device() == device, "k_cache and v_cache must be on CUDA, on the device of the other tensors");
+    TORCH_CHECK(t->dim() == 4 && t->size(2) == heads && t->size(3) == head_dim,
+                "k_cache and v_cache must have shape (num_pages, page_size, num_heads, head_size)");
+    TORCH_CHECK(t->scalar_type() == (e4m3 ? at::kFloat8_e4m3fn : type),
+                "k_cache and v_cache must both be of the type of the other tensors, or both float8_e4m3fn");
+    TORCH_CHECK(t->stride(-1) == 1, "k_cache and v_cache must have contiguous last dimension");
+  }
+  TORCH_CHECK(v_cache.sizes() == k_cache.sizes(), "v_cache must have the shape of k_cache");
+  TORCH_CHECK(k_cache.size(0) > 0 && k_cache.size(1) > 0 && k_cache.size(1) % 16 == 0,
+              "k_cache and v_cache must hold at least one page, of a multiple of 16 tokens, got ", k_cache.size(0),
+              " of ", k_cache.size(1));
+  TORCH_CHECK(k_scale.has_value() == e4m3 && v_scale.has_value() == e4m3,
+              "k_scale and v_scale belong to float8_e4m3fn caches, and only to them");
+  if (e4m3) {
+    for (const OptTensor* t : {&k_scale, &v_scale})
+      TORCH_CHECK((*t)->is_cuda() && (*t)->device() == device && (*t)->dim() == 3 &&
+                      (*t)->sizes() == k_cache.sizes().slice(0, 3) &&
+                      ((*t)->scalar_type() == at::kFloat8_e8m0fnu || (*t)->scalar_type() == at::kByte),
+                  "k_scale and v_scale must be float8_e8m0fnu (or uint8) CUDA tensors (num_pages, page_size, num_heads)");
+    c.k_scale = static_cast<uint8_t*>(k_scale->data_ptr());
+    c.v_scale = static_cast<uint8_t*>(v_scale->data_ptr());
+    c.k_scale_strides = strides_of(*k_scale);
+    c.v_scale_strides = strides_of(*v_scale);
+  }
+  TORCH_CHECK(block_table.is_cuda() && block_table.device() == device && block_table.scalar_type() == at::kInt &&
+                  block_table.dim() == 2 && block_table.size(0) == batch && block_table.size(1) > 0 &&
+                  (block_table.size(1) == 1 || block_table.stride(1) == 1),
+              "block_table must be an int32 CUDA tensor (batch_size, max_pages) with contiguous rows");
+  c.k = k_cache.data_ptr();
+  c.v = v_cache.data_ptr();
+  c.k_strides = strides_of(k_cache);
+  c.v_strides = strides_of(v_cache);
+  c.block_table = block_table.data_ptr<int32_t>();
+  c.block_table_stride = block_table.stride(0);
+  c.num_pages = int32_of(k_cache.size(0), "num_pages");
+  c.page_size = int32_of(k_cache.size(1), "page_size");
+  c.max_pages = int32_of(block_table.size(1), "max_pages");
+  c.format = e4m3 ? FMHA_CACHE_E4M3 : FMHA_CACHE_16BIT;
+  return c;
+}
+
+const int32_t* lengths_ptr(const at::Tensor& t, int64_t batch, c10::Device device, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == device && t.scalar_type() == at::kInt && t.dim() == 1 &&
+                  t.size(0) == batch && t.is_contiguous(),
+              name, " must be a contiguous int32 CUDA tensor with one entry per batch");
+  return t.data_ptr<int32_t>();
+}
+
+int32_t dtype_code(at::ScalarType type) { return type == at::kBFloat16 ? FMHA_DTYPE_BF16 : FMHA_DTYPE_FP16; }
+
+void op_paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                    const at::Tensor& block_table, const at::Tensor& cache_seqlens, const OptTensor& seqused,
+                    const OptTensor& k_scale, const OptTensor& v_scale) {
+  check_input(k, "k");
+  check_input(v, "v");
+  TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
+              "v must have the shape, type and device of k");
+  FmhaCacheWriteParams p = {};
+  p.cache = cache_of(k_cache, v_cache, block_table, k_scale, v_scale, k.scalar_type(), k.device(), k.size(0),
+                     k.size(2), k.size(3));
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.k_strides = strides_of(k);
+  p.v_strides = strides_of(v);
+  p.seqlens = lengths_ptr(cache_seqlens, k.size(0), k.device(), "cache_seqlens");
+  if (seqused.has_value()) p.seqused = lengths_ptr(*seqused, k.size(0), k.device(), "seqused");
+  p.batch = int32_of(k.size(0), "batch_size");
+  p.seqlen = int32_of(k.size(1), "seqlen");
+  p.heads = int32_of(k.size(2), "num_heads");
+  p.head_dim = int32_of(k.size(3), "head_size");
+  p.dtype = dtype_code(k.scalar_type());
+  c10::cuda::CUDAGuard guard(k.device());
+  check_status(fmha_cache_write(&p, at::cuda::getCurrentCUDAStream().stream()), "fmha_cache_write");
+}
+
+std::tuple<at::Tensor, at::Tensor> op_paged_read(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                 const at::Tensor& block_table, const at::Tensor& seqused_k,
+                                                 int64_t seqlen, const OptTensor& k_scale, const OptTensor& v_scale,
+                                                 at::ScalarType dtype) {
+  TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "This repo only supports fp16 and bf16 data types (dtype)");
+  TORCH_CHECK(k_cache.dim() == 4, "k_cache and v_cache must have shape (num_pages, page_size, num_heads, head_size)");
+  TORCH_CHECK(seqlen >= 0, "seqlen must not be negative");
+  const int64_t batch = block_table.dim() > 0 ? block_table.size(0) : 0;
+  FmhaCacheReadParams p = {};
+  p.cache = cache_of(k_cache, v_cache, block_table, k_scale, v_scale, dtype, k_cache.device(), batch,
+                     k_cache.size(2), k_cache.size(3));
+  p.seqused_k = lengths_ptr(seqused_k, batch, k_cache.device(), "seqused_k");
+  p.batch = int32_of(batch, "batch_size");
+  p.seqlen = int32_of(seqlen, "seqlen");
+  p.heads = int32_of(k_cache.size(2), "num_heads");
+  p.head_dim = int32_of(k_cache.size(3), "head_size");
+  p.dtype = dtype_code(dtype);
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  const int64_t sizes[4] = {batch, seqlen, k_cache.size(2), k_cache.size(3)};
+  at::Tensor k = empty_on(k_cache, sizes, dtype), v = empty_on(k_cache, sizes, dtype);
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.k_strides = strides_of(k);
+  p.v_strides = strides_of(v);
+  check_status(fmha_cache_read(&p, at::cuda::getCurrentCUDAStream().stream()), "fmha_cache_read");
+  return {k, v};
+}
+
+std::tuple<at::Tensor, at::Tensor> op_paged_fwd(const at::Tensor& q, const at::Tensor& k_cache,
+                                                const at::Tensor& v_cache, const at::Tensor& block_table,
+                                                const at::Tensor& seqused_k, const OptTensor& seqused_q,
+                                                const OptTensor& k_scale, const OptTensor& v_scale,
+                                                double softmax_scale, bool causal) {
+  check_input(q, "q");
+  TORCH_CHECK(k_cache.dim() == 4, "k_cache and v_cache must have shape (num_pages, page_size, num_heads, head_size)");
+  const int64_t B = q.size(0), Nq = q.size(1), Hq = q.size(2), D = q.size(3), Hk = k_cache.size(2);
+  TORCH_CHECK(Hk > 0 && Hq > 0 && Hq % Hk == 0 && Hq / Hk <= 128,
+              "q must have a multiple of the cache's heads, 128 times as many at most, got ", Hq, " and ", Hk);
+  FmhaPagedFwdParams p = {};
+  p.cache = cache_of(k_cache, v_cache, block_table, k_scale, v_scale, q.scalar_type(), q.device(), B, Hk, D);
+  p.seqused_k = lengths_ptr(seqused_k, B, q.device(), "seqused_k");
+  if (seqused_q.has_value()) p.seqused_q = lengths_ptr(*seqused_q, B, q.device(), "seqused_q");
+  p.q = q.data_ptr();
+  p.q_strides = strides_of(q);
+  p.batch = int32_of(B, "batch_size");
+  p.seqlen_q = int32_of(Nq, "seqlen_q");
+  p.heads_q = int32_of(Hq, "num_heads");
+  p.heads_k = int32_of(Hk, "num_heads");
+  p.head_dim = int32_of(D, "head_size");
+  p.dtype = dtype_code(q.scalar_type());
+  p.scale = static_cast<float>(softmax_scale);
+  p.causal = causal ? 1 : 0;
+  c10::cuda::CUDAGuard guard(q.device());
+  // rows without gaps, so that the strides are what the kernels can take whatever q's are
+  at::Tensor out = empty_on(q, q.sizes(), q.scalar_type()), lse = empty_on(q, {B, Hq, Nq}, at::kFloat);
+  p.o = out.data_ptr();
+  p.o_strides = strides_of(out);
+  p.lse = lse.data_ptr<float>();
+  const size_t ws_bytes = fmha_paged_fwd_workspace_bytes(&p);
+  at::Tensor ws;
+  if (ws_bytes > 0) ws = empty_on(q, {static_cast<int64_t>(ws_bytes)}, at::kByte);
+  check_status(fmha_paged_fwd(&p, ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes,
+                              at::cuda::getCurrentCUDAStream().stream()),
+               "fmha_paged_fwd");
+  return {out, lse};
+}
+
+// The cache serves; none of its functions has a derivative, and what autograd would have to know is refused
+// instead of dropped.
+void check_no_derivative(std::initializer_list<const at::Tensor*> inputs, const char* name) {
+  if (const auto& functorch = at::functorch::functorchTLSAccessor()) functorch->checkSupportsCppAutogradFunction();
+  for (const at::Tensor* t : inputs) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()), name,
+                " has no derivative: call it under torch.no_grad(), or on inputs that require none");
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), name,
+                                  " has no forward-mode derivative (an input carries a tangent)");
+  }
+}
+
+// flash_attn_paged_func, paged_cache_write and paged_cache_read outside of tracing
+std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k_cache,
+                                                   const at::Tensor& v_cache, const at::Tensor& block_table,
+                                                   const at::Tensor& seqused_k, const OptTensor& seqused_q,
+                                                   const OptTensor& k_scale, const OptTensor& v_scale,
+                                                   std::optional<double> softmax_scale, bool causal) {
+  TORCH_CHECK(q.dim() > 0, "q must have shape (batch, seqlen, heads, head_size)");
+  check_no_derivative({&q, &k_cache, &v_cache}, "flash_attn_paged_func");
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("flash_attn_v100::paged_fwd", "")
+                             .typed<decltype(op_paged_fwd)>();
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(last_dim_contiguous(q), k_cache, v_cache, block_table, seqused_k, seqused_q, k_scale, v_scale,
+                 softmax_scale.has_value() ? *softmax_scale : std::pow((double)q.size(-1), -0.5), causal);
+}
+
+void paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                 const at::Tensor& block_table, const at::Tensor& cache_seqlens, const OptTensor& seqused,
+                 const OptTensor& k_scale, const OptTensor& v_scale) {
+  check_no_derivative({&k, &v, &k_cache, &v_cache}, "paged_cache_write");
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("flash_attn_v100::paged_write", "")
+                             .typed<decltype(op_paged_write)>();
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    op.call(last_dim_contiguous(k), last_dim_contiguous(v), k_cache, v_cache, block_table, cache_seqlens, seqused,
+            k_scale, v_scale);
+  }
+  // what autograd saved of these tensors before is no longer what they hold
+  // (tensors made under inference_mode keep no count)
+  auto written = [](const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  written(k_cache);
+  written(v_cache);
+  if (k_scale.has_value()) written(*k_scale);
+  if (v_scale.has_value()) written(*v_scale);
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                              const at::Tensor& block_table, const at::Tensor& seqused_k,
+                                              int64_t seqlen, const OptTensor& k_scale, const OptTensor& v_scale,
+                                              at::ScalarType dtype) {
+  check_no_derivative({&k_cache, &v_cache}, "paged_cache_read");
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("flash_attn_v100::paged_read", "")
+                             .typed<decltype(op_paged_read)>();
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(k_cache, v_cache, block_table, seqused_k, seqlen, k_scale, v_scale, dtype);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(flash_attn_v100, m) {
@@ -381,16 +603,29 @@ TORCH_LIBRARY(flash_attn_v100, m) {
   m.def("bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor softmax_lse, float softmax_scale, "
         "bool causal, Tensor? seqused_q=None, Tensor? seqused_k=None, bool deterministic=False) -> (Tensor, "
         "Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+  m.def("paged_write(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor cache_seqlens, "
+        "Tensor? seqused=None, Tensor(c!)? k_scale=None, Tensor(d!)? v_scale=None) -> ()", {at::Tag::pt2_compliant_tag});
+  m.def("paged_read(Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seqused_k, int seqlen, Tensor? k_scale=None, "
+        "Tensor? v_scale=None, *, ScalarType dtype) -> (Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+  m.def("paged_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seqused_k, Tensor? seqused_q, "
+        "Tensor? k_scale, Tensor? v_scale, float softmax_scale, bool causal) -> (Tensor, Tensor)",
+        {at::Tag::pt2_compliant_tag});
 }
 TORCH_LIBRARY_IMPL(flash_attn_v100, CUDA, m) {
   m.impl("fwd", TORCH_FN(op_fwd));
   m.impl("bwd", TORCH_FN(op_bwd));
+  m.impl("paged_write", TORCH_FN(op_paged_write));
+  m.impl("paged_read", TORCH_FN(op_paged_read));
+  m.impl("paged_fwd", TORCH_FN(op_paged_fwd));
 }
 // the ops themselves have no derivative (the functions above do): differentiating through a direct
 // call is an error, not a silent zero
 TORCH_LIBRARY_IMPL(flash_attn_v100, Autograd, m) {
   m.impl("fwd", torch::autograd::autogradNotImplementedFallback());
   m.impl("bwd", torch::autograd::autogradNotImplementedFallback());
+  m.impl("paged_write", torch::autograd::autogradNotImplementedFallback());
+  m.impl("paged_read", torch::autograd::autogradNotImplementedFallback());
+  m.impl("paged_fwd", torch::autograd::autogradNotImplementedFallback());
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -409,5 +644,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention", &attention,
         "Attention with autograd: attention(q, k, v, softmax_scale|None, causal, seqused_q|None, "
         "seqused_k|None, deterministic)");
+  m.def("paged_attention", &paged_attention,
+        "Attention over a paged cache, [out, lse]: paged_attention(q, k_cache, v_cache, block_table, seqused_k, "
+        "seqused_q|None, k_scale|None, v_scale|None, softmax_scale|None, causal)");
+  m.def("paged_write", &paged_write,
+        "New tokens into a paged cache: paged_write(k, v, k_cache, v_cache, block_table, cache_seqlens, seqused|None, "
+        "k_scale|None, v_scale|None)");
+  m.def("paged_read", &paged_read,
+        "Tokens out of a paged cache, [k, v]: paged_read(k_cache, v_cache, block_table, seqused_k, seqlen, k_scale|None, "
+        "v_scale|None, dtype)");
   m.def("version", []() { return std::string(fmha_version()); });
 }

@@ -5,4 +5,7 @@ __version__ = "0.3.0"
 from flash_attn_v100.flash_attn_interface import (  # noqa: F401
     flash_attn_func,
     flash_attn_padded_func,
+    flash_attn_paged_func,
+    paged_cache_read,
+    paged_cache_write,
 )

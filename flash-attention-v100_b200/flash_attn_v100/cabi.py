@@ -35,6 +35,7 @@ EXPORTED_SYMBOLS = (
     "fmha_b200_backward", "fmha_status_string", "fmha_version",
     "fmha_ipc_export", "fmha_ipc_open", "fmha_ipc_close", "fmha_peer_copy", "fmha_peer_copy_2d",
     "fmha_counter_bump", "fmha_peer_signal", "fmha_peer_wait", "fmha_sum_partials", "fmha_merge_parts",
+    "fmha_cache_write", "fmha_cache_read", "fmha_paged_fwd", "fmha_paged_fwd_workspace_bytes",
 )
 
 
@@ -72,6 +73,51 @@ class FmhaBwdParams(ctypes.Structure):
         ("flags", ctypes.c_int32), ("status", ctypes.c_void_p), ("dtype", ctypes.c_int32),
         ("seqused_q", ctypes.c_void_p), ("seqused_k", ctypes.c_void_p),
         ("q_row_begin", ctypes.c_int32),
+    ]
+
+
+FMHA_CACHE_16BIT = 0
+FMHA_CACHE_E4M3 = 1
+
+
+class FmhaPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int64),
+        ("k_strides", FmhaStrides), ("v_strides", FmhaStrides), ("k_scale_strides", FmhaStrides),
+        ("v_scale_strides", FmhaStrides),
+        ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+        ("format", ctypes.c_int32),
+    ]
+
+
+class FmhaCacheWriteParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", FmhaPagedCache), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_strides", FmhaStrides), ("v_strides", FmhaStrides),
+        ("seqlens", ctypes.c_void_p), ("seqused", ctypes.c_void_p),
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("seqlen", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
+class FmhaCacheReadParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", FmhaPagedCache), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_strides", FmhaStrides), ("v_strides", FmhaStrides), ("seqused_k", ctypes.c_void_p),
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("seqlen", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
+class FmhaPagedFwdParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", FmhaPagedCache), ("q", ctypes.c_void_p), ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("q_strides", FmhaStrides), ("o_strides", FmhaStrides),
+        ("seqused_k", ctypes.c_void_p), ("seqused_q", ctypes.c_void_p),
+        ("batch", ctypes.c_int32), ("heads_q", ctypes.c_int32), ("heads_k", ctypes.c_int32),
+        ("seqlen_q", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("causal", ctypes.c_int32), ("status", ctypes.c_void_p),
     ]
 
 
@@ -136,6 +182,13 @@ def load_library() -> ctypes.CDLL:
                                   ctypes.POINTER(i32), i32, vp, vp, i32, i32, i32, i32, i32, vp])):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = args
+    for name, params in (("fmha_cache_write", FmhaCacheWriteParams), ("fmha_cache_read", FmhaCacheReadParams)):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [ctypes.POINTER(params), vp]
+    lib.fmha_paged_fwd.restype = ctypes.c_int
+    lib.fmha_paged_fwd.argtypes = [ctypes.POINTER(FmhaPagedFwdParams), vp, sz, vp]
+    lib.fmha_paged_fwd_workspace_bytes.restype = sz
+    lib.fmha_paged_fwd_workspace_bytes.argtypes = [ctypes.POINTER(FmhaPagedFwdParams)]
     lib.fmha_status_string.restype = ctypes.c_char_p
     lib.fmha_status_string.argtypes = [ctypes.c_int]
     lib.fmha_version.restype = ctypes.c_char_p
@@ -437,3 +490,42 @@ def merge_parts(o_parts, lse_parts, row_offsets, o_out, lse_out, stream=None):
                                                _ptr(o_out), _ptr(lse_out), Z, H, rows, D,
                                                _dtype_code(o_out), _stream(stream)), "fmha_merge_parts")
     return o_out, lse_out
+
+
+def paged_cache(k_cache, v_cache, block_table, k_scale=None, v_scale=None) -> FmhaPagedCache:
+    """The C struct for pools (num_pages, page_size, heads, head_dim) and their block table."""
+    c = FmhaPagedCache()
+    c.k, c.v, c.block_table = k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr()
+    c.block_table_stride = block_table.stride(0)
+    c.k_strides, c.v_strides = _strides(k_cache), _strides(v_cache)
+    if k_scale is not None:
+        c.format = FMHA_CACHE_E4M3
+        c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        c.k_scale_strides, c.v_scale_strides = _strides(k_scale), _strides(v_scale)
+    c.num_pages, c.page_size, c.max_pages = k_cache.shape[0], k_cache.shape[1], block_table.shape[1]
+    return c
+
+
+def paged_fwd(q, cache: FmhaPagedCache, heads_k: int, seqused_k, scale: float, causal: bool = False, seqused_q=None,
+              status=None, workspace=None, out=None, lse=None, stream=None):
+    """O, LSE through ``fmha_paged_fwd``; outputs and workspace allocated with torch unless passed in."""
+    _require_cuda_half(q, out)
+    Z, N, H, D = q.shape
+    out = torch.empty((Z, N, H, D), dtype=q.dtype, device=q.device) if out is None else out
+    lse = torch.empty((Z, H, N), dtype=torch.float32, device=q.device) if lse is None else lse
+    p = FmhaPagedFwdParams()
+    p.cache, p.q, p.o, p.lse = cache, q.data_ptr(), out.data_ptr(), lse.data_ptr()
+    p.q_strides, p.o_strides = _strides(q), _strides(out)
+    p.seqused_k, p.seqused_q = _seqused_ptr(seqused_k, Z), _seqused_ptr(seqused_q, Z)
+    p.batch, p.seqlen_q, p.heads_q, p.head_dim = Z, N, H, D
+    p.heads_k = heads_k
+    p.dtype, p.scale, p.causal = _dtype_code(q), float(scale), int(bool(causal))
+    p.status = None if status is None else status.data_ptr()
+    lib = load_library()
+    with torch.cuda.device(q.device):
+        if workspace is None:
+            nbytes = int(lib.fmha_paged_fwd_workspace_bytes(ctypes.byref(p)))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _check(lib.fmha_paged_fwd(ctypes.byref(p), _ptr(workspace), workspace.numel() * workspace.element_size(),
+                                  _stream(stream)), "fmha_paged_fwd")
+    return out, lse

@@ -144,3 +144,83 @@ def flash_attn_func(q, k, v, softmax_scale: Optional[float] = None, causal: bool
     if torch.compiler.is_compiling():
         return FlashAttnFunc.apply(q, k, v, softmax_scale, causal)
     return flash_attn_cuda.attention(q, k, v, softmax_scale, causal, None, None, False)
+
+
+# ------------------------------------------------------------------------------------------------
+# A paged key/value cache and the attention over it (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------------
+@torch.library.register_fake("flash_attn_v100::paged_write")
+def _paged_write_fake(k, v, k_cache, v_cache, block_table, cache_seqlens, seqused=None, k_scale=None, v_scale=None):
+    return None
+
+
+@torch.library.register_fake("flash_attn_v100::paged_read")
+def _paged_read_fake(k_cache, v_cache, block_table, seqused_k, seqlen, k_scale=None, v_scale=None, *, dtype):
+    shape = (block_table.shape[0], seqlen, k_cache.shape[2], k_cache.shape[3])
+    return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+
+
+@torch.library.register_fake("flash_attn_v100::paged_fwd")
+def _paged_fwd_fake(q, k_cache, v_cache, block_table, seqused_k, seqused_q, k_scale, v_scale, softmax_scale, causal):
+    Z, N, H, _ = q.shape
+    return q.new_empty(q.shape), q.new_empty((Z, H, N), dtype=torch.float32)
+
+
+def paged_cache_write(k, v, k_cache, v_cache, block_table, cache_seqlens, seqused=None, k_scale=None,
+                      v_scale=None) -> None:
+    """New tokens' K and V into a paged cache, in place.
+
+    k, v: fp16 or bf16 CUDA tensors (batch, new tokens, heads, head_dim).  k_cache, v_cache: (num_pages,
+    page_size, heads, head_dim), page_size a multiple of 16, of the same type, or float8_e4m3fn with k_scale and
+    v_scale (num_pages, page_size, heads) of float8_e8m0fnu: a token's head is then rounded to 8 bits under
+    the smallest power of two that holds its largest value (values that are not finite become NaN).
+    block_table: int32 (batch, max_pages); token t of entry z is row t % page_size of page
+    block_table[z, t // page_size].  cache_seqlens: int32 (batch,), tokens an entry holds already; its new
+    ones follow them.  seqused: int32 (batch,) or None, how many of the new tokens are real.  What goes beyond
+    an entry's pages, or to a page that the pool does not have, is dropped.
+    """
+    if torch.compiler.is_compiling():
+        torch.ops.flash_attn_v100.paged_write(_maybe_contiguous(k), _maybe_contiguous(v), k_cache, v_cache, block_table,
+                                              cache_seqlens, seqused, k_scale, v_scale)
+        return
+    flash_attn_cuda.paged_write(k, v, k_cache, v_cache, block_table, cache_seqlens, seqused, k_scale, v_scale)
+
+
+def paged_cache_read(k_cache, v_cache, block_table, seqused_k, seqlen: Optional[int] = None, k_scale=None, v_scale=None,
+                     dtype: Optional[torch.dtype] = None):
+    """K and V (batch, seqlen, heads, head_dim) out of a paged cache: the first ``seqlen`` tokens of every
+    entry, zeros from token seqused_k[z] on.  ``seqlen`` defaults to what the block table has room for, ``dtype``
+    to the cache's; a float8_e4m3fn cache needs one (fp16 or bf16; in the type that was written from, what the 8
+    bits stand for is exact)."""
+    if seqlen is None:
+        seqlen = block_table.shape[1] * k_cache.shape[1]
+    if dtype is None:
+        dtype = k_cache.dtype
+    if torch.compiler.is_compiling():
+        return torch.ops.flash_attn_v100.paged_read(k_cache, v_cache, block_table, seqused_k, seqlen, k_scale, v_scale,
+                                                    dtype=dtype)
+    return flash_attn_cuda.paged_read(k_cache, v_cache, block_table, seqused_k, seqlen, k_scale, v_scale, dtype)
+
+
+def flash_attn_paged_func(q, k_cache, v_cache, block_table, seqused_k, seqused_q=None, k_scale=None, v_scale=None,
+                          softmax_scale: Optional[float] = None, causal: bool = False, return_lse: bool = False):
+    """Attention of new tokens over a paged cache that holds their K and V and all before them.
+
+    q: fp16 or bf16 (batch, new tokens, query heads, head_dim), head_dim 64, 96 or 128, any number of tokens;
+    query heads a multiple of the cache's (query head h reads head h // (query heads // heads)).  The cache, its
+    block table and scales are those of ``paged_cache_write``.  seqused_k: int32 (batch,), tokens of an entry in
+    the cache, its new ones among them (the call follows ``paged_cache_write``: cache_seqlens plus the new ones).
+    seqused_q: int32 (batch,) or None, how many of q's tokens are real.  With ``causal``, new token i of entry z sees
+    the keys j <= seqused_k[z] - seqused_q[z] + i.  Returns (batch, new tokens, query heads, head_dim), zeros
+    where a token sees nothing or is padding, with ``return_lse`` also the log-sum-exp (batch, query heads,
+    new tokens) in fp32, -inf there.  Lengths and pages are read on the device: a captured call follows them.
+    Has no derivative.
+    """
+    if torch.compiler.is_compiling():
+        scale = q.shape[-1] ** (-0.5) if softmax_scale is None else float(softmax_scale)
+        out, lse = torch.ops.flash_attn_v100.paged_fwd(_maybe_contiguous(q), k_cache, v_cache, block_table, seqused_k,
+                                                       seqused_q, k_scale, v_scale, scale, causal)
+    else:
+        out, lse = flash_attn_cuda.paged_attention(q, k_cache, v_cache, block_table, seqused_k, seqused_q, k_scale,
+                                                   v_scale, softmax_scale, causal)
+    return (out, lse) if return_lse else out

@@ -335,6 +335,92 @@ int fmha_merge_parts(const void* const* o_parts, const float* const* lse_parts,
                      void* o_out, float* lse_out, int32_t batch, int32_t heads, int32_t rows,
                      int32_t head_dim, int32_t dtype, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * A paged key/value cache, and attention over it.  None of it has a counterpart in the reference.
+ *
+ * The cache is two pools of pages, K and V, of shape (num_pages, page_size, H, D): a page holds
+ * page_size (a multiple of 16) consecutive tokens of one batch entry.  Row z of the block table names
+ * entry z's pages in order: token t is row t % page_size of page block_table[z][t / page_size], and an entry
+ * holds at most max_pages * page_size tokens.  Pools may be strided (pages, rows and heads in any order).
+ *
+ * Formats: FMHA_CACHE_16BIT holds the elements of `dtype`.  FMHA_CACHE_E4M3 holds one byte per element
+ * and one byte of scale per token and head: an element is code * 2^(scale byte - 127).  The exponent is the
+ * smallest for which the row's largest finite magnitude is at most 448 * 2^e, within [-15, 8] for fp16 and
+ * [-120, 120] for bf16: what a row stands for is then exact in the type it was written from (a power of two
+ * costs a floating code nothing), so whoever reads it adds no rounding.  Codes are rounded to nearest, halves
+ * to even; values that are not finite become NaN, which e4m3 has; a value that would round to 2^16
+ * (bf16: 2^128) is rounded towards zero instead.
+ *
+ * A block-table entry outside [0, num_pages) is no page: nothing is written there, and its tokens are
+ * read as zeros.  Entries behind an entry's last token are not looked at.
+ * ------------------------------------------------------------------------------------------ */
+#define FMHA_CACHE_16BIT 0
+#define FMHA_CACHE_E4M3 1
+
+typedef struct {
+  void* k; /* pools; written by fmha_cache_write only */
+  void* v;
+  uint8_t* k_scale; /* FMHA_CACHE_E4M3: (num_pages, page_size, H) bytes; not looked at otherwise */
+  uint8_t* v_scale;
+  const int32_t* block_table;   /* device, `batch` rows of max_pages entries */
+  int64_t block_table_stride;   /* entries between its rows (>= max_pages) */
+  /* `batch` is the stride between pages; in elements, multiples of 16 bytes.  The scales' may be anything. */
+  FmhaStrides k_strides, v_strides, k_scale_strides, v_scale_strides;
+  int32_t num_pages, page_size, max_pages;
+  int32_t format; /* FMHA_CACHE_* */
+} FmhaPagedCache;
+
+typedef struct {
+  FmhaPagedCache cache;
+  const void* k; /* new tokens (Z, seqlen, H, D) of `dtype` */
+  const void* v;
+  FmhaStrides k_strides, v_strides;
+  const int32_t* seqlens;  /* (Z) device: tokens an entry holds already; new token i goes to seqlens[z] + i */
+  const int32_t* seqused;  /* (Z) device or NULL: new tokens of entry z that are real (all seqlen) */
+  int32_t batch, heads, seqlen, head_dim, dtype;
+} FmhaCacheWriteParams;
+
+/* New tokens' K and V into their pages.  Tokens behind an entry's capacity are dropped; two tokens of a call at
+ * one place leave either of them, row by row.  seqlen = 0 or batch = 0 does nothing. */
+int fmha_cache_write(const FmhaCacheWriteParams* p, void* stream);
+
+typedef struct {
+  FmhaPagedCache cache;
+  void* k; /* (Z, seqlen, H, D) of `dtype`, written */
+  void* v;
+  FmhaStrides k_strides, v_strides;
+  const int32_t* seqused_k; /* (Z) device: tokens an entry holds */
+  int32_t batch, heads, seqlen, head_dim, dtype;
+} FmhaCacheReadParams;
+
+/* Tokens [0, seqlen) of every entry out of their pages, zeros behind an entry's last token.  From
+ * FMHA_CACHE_E4M3 to another type than the one written from, values are rounded to nearest. */
+int fmha_cache_read(const FmhaCacheReadParams* p, void* stream);
+
+typedef struct {
+  FmhaPagedCache cache;
+  const void* q; /* (Z, seqlen_q, heads_q, D) */
+  void* o;       /* like q, written; padding rows are zeros */
+  float* lse;    /* (Z, heads_q, seqlen_q) fp32, written; padding rows are -inf */
+  FmhaStrides q_strides, o_strides;
+  const int32_t* seqused_k; /* (Z) device: tokens of an entry in the cache, its new ones among them */
+  const int32_t* seqused_q; /* (Z) device or NULL: new tokens of entry z (all seqlen_q) */
+  int32_t batch, heads_q, heads_k; /* heads_q = a multiple of heads_k (128 times at most); query head h reads head
+                                      h / (heads_q / heads_k) of the cache */
+  int32_t seqlen_q, head_dim, dtype;
+  float scale;
+  int32_t causal; /* 1: new token i of entry z sees the keys j <= seqused_k[z] - seqused_q[z] + i */
+  int32_t* status;
+} FmhaPagedFwdParams;
+
+/* Attention of new tokens over the cache that holds their K and V (and whatever came before): O and LSE as
+ * fmha_fwd has them.  Lengths are read on the device, so a captured call follows them.  Cached rows behind an
+ * entry's last token may hold anything, NaN included.  Work is cut evenly over the SMs and what was cut is joined:
+ * that takes `workspace` (device, 16-byte aligned, of fmha_paged_fwd_workspace_bytes(p) bytes, which depends on sizes
+ * only; its contents mean nothing before or after, and calls that may overlap need one each). */
+size_t fmha_paged_fwd_workspace_bytes(const FmhaPagedFwdParams* p);
+int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Reference-shaped launchers: same argument meaning as include/fused_mha.h:1-6, dense fp16
  * (batch, m|n, head, k) tensors, except that the `max`/`sum` pair becomes one `lse` buffer,
  * the backward's `d_ptr` (fp16 D) is dropped in favour of a caller workspace, and a status
