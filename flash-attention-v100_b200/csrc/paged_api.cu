@@ -6,10 +6,13 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <numeric>
+#include <type_traits>
 
 #include "../../include/fmha_b200.h"
 #include "cache_kernels.cuh"
 #include "host_common.cuh"
+#include "paged_few_kernel.cuh"
 #include "paged_simple_kernel.cuh"
 
 namespace {
@@ -97,6 +100,142 @@ fmha::PagedCache device_cache(const FmhaPagedCache& c) {
     FMHA_DISPATCH_CACHE_FORMAT(dtype, format, __VA_ARGS__)             \
   }
 
+// A pool as a 4-D map (D, page_size, H, num_pages), box 64 x box_rows x 1 x 1, 128-byte swizzle, zeros outside
+int make_pool_map(CUtensorMap* map, const void* base, const FmhaPagedCache& c, const FmhaStrides& s, int heads, int D,
+                  int box_rows, bool bf16) {
+  EncodeTiledFn encode = get_encode_fn();
+  if (encode == nullptr) return FMHA_ERR_NO_DEVICE;
+  // a stride of a size-1 dimension is never used for addressing; make it well-formed
+  const int64_t row = s.row, head = heads > 1 ? s.head : D;
+  const int64_t page = c.num_pages > 1 ? s.batch : row * c.page_size;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)c.page_size, (cuuint64_t)heads, (cuuint64_t)c.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FMHA_OK : FMHA_ERR_TENSOR_MAP;
+}
+
+// Rows of one cache head's queries, (Z, N, H, D) as a 4-D map (D, H, N, Z), box 64 x heads x tokens x 1: the box's rows
+// are tokens with a cache head's query heads inside
+int make_rows_map(CUtensorMap* map, const void* base, int Z, int N, int H, int D, const FmhaStrides& s, int heads, int tokens,
+                  bool bf16) {
+  EncodeTiledFn encode = get_encode_fn();
+  if (encode == nullptr) return FMHA_ERR_NO_DEVICE;
+  const int64_t head = H > 1 ? s.head : D, row = N > 1 ? s.row : head * H;
+  const int64_t batch = Z > 1 ? s.batch : row * N;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)N, (cuuint64_t)Z};
+  const cuuint64_t strides[3] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2, (cuuint64_t)batch * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)heads, (cuuint32_t)tokens, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FMHA_OK : FMHA_ERR_TENSOR_MAP;
+}
+
+// How a call is cut (paged_work.cuh) and what that takes.
+struct PagedPlan {
+  int kernel_rows;       // rows of an item that the kernel has room for
+  int tokens_per_block;  // new tokens of an item
+  int blocks_per_entry;
+  int min_share;
+  int blocks;            // of the grid
+  size_t part_bytes, lse_bytes, item_bytes;
+  size_t bytes() const { return part_bytes + lse_bytes + item_bytes; }
+};
+
+// Rows of up to 16, 32 or 64 run the kernel of few rows.
+PagedPlan plan_paged(const FmhaPagedFwdParams* p, int sms) {
+  PagedPlan plan = {};
+  const int group = p->heads_q / p->heads_k;
+  const long long rows = (long long)p->seqlen_q * group;
+  if (rows > 64) return plan;
+  plan.kernel_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  plan.tokens_per_block = p->seqlen_q;
+  plan.blocks_per_entry = 1;
+  plan.min_share = 2;
+  plan.blocks = sms;
+  const size_t items = (size_t)p->batch * plan.blocks_per_entry * p->heads_k;
+  plan.part_bytes = (size_t)2 * plan.blocks * plan.kernel_rows * p->head_dim * sizeof(float);
+  plan.lse_bytes = ((size_t)2 * plan.blocks * plan.kernel_rows * sizeof(float) + 255) / 256 * 256;
+  plan.item_bytes = items * sizeof(int2);
+  return plan;
+}
+
+fmha::PagedParams kernel_params(const FmhaPagedFwdParams* p, const PagedPlan& plan, void* workspace) {
+  fmha::PagedParams a;
+  a.cache = device_cache(p->cache);
+  a.seqused_k = p->seqused_k;
+  a.seqused_q = p->seqused_q;
+  a.batch = p->batch;
+  a.heads_k = p->heads_k;
+  a.group = p->heads_q / p->heads_k;
+  a.seqlen_q = p->seqlen_q;
+  a.causal = p->causal ? 1 : 0;
+  a.blocks_per_entry = plan.blocks_per_entry;
+  a.tokens_per_block = plan.tokens_per_block;
+  a.box_rows = std::gcd(p->cache.page_size, 128);
+  a.min_share = plan.min_share;
+  a.scale_log2 = std::fabs(p->scale) * 1.4426950408889634f;
+  a.negate = p->scale < 0.f;
+  a.o = static_cast<uint16_t*>(p->o);
+  a.o_batch = p->o_strides.batch;
+  a.o_row = p->o_strides.row;
+  a.o_head = p->o_strides.head;
+  a.lse = p->lse;
+  char* ws = static_cast<char*>(workspace);
+  a.o_part = reinterpret_cast<float*>(ws);
+  a.lse_part = reinterpret_cast<float*>(ws + plan.part_bytes);
+  a.item_blocks = reinterpret_cast<int2*>(ws + plan.part_bytes + plan.lse_bytes);
+  a.status = p->status;
+  return a;
+}
+
+// joins what was cut, launched as soon as no block of the kernel before is left to start or run (it waits for
+// their writes itself)
+template <bool kBf16, int DR, int kRows>
+int launch_join(const fmha::PagedParams& a, const PagedPlan& plan, int rows_per_item, cudaStream_t stream) {
+  using E = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+  const int items = a.batch * a.blocks_per_entry * a.heads_k;
+  const long long rows = (long long)items * rows_per_item;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)((rows + 7) / 8));
+  config.blockDim = dim3(256);
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, fmha::paged_join_kernel<E, DR, kRows>, a, rows_per_item, items, plan.blocks) !=
+      cudaSuccess) {
+    (void)cudaGetLastError();
+    return FMHA_ERR_LAUNCH;
+  }
+  return FMHA_OK;
+}
+
+template <int D, int DR, bool kBf16, bool kE4m3, int kRows>
+int launch_few(const FmhaPagedFwdParams* p, const PagedPlan& plan, void* workspace, int dev, cudaStream_t stream) {
+  using T = fmha::FewTraits<D, DR, kBf16, kE4m3, kRows>;
+  const fmha::PagedParams a = kernel_params(p, plan, workspace);
+  CUtensorMap tq, tk = {}, tv = {};
+  int rc;
+  if ((rc = make_rows_map(&tq, p->q, p->batch, p->seqlen_q, p->heads_q, DR, p->q_strides, a.group, p->seqlen_q, kBf16)))
+    return rc;
+  if (!kE4m3 &&
+      ((rc = make_pool_map(&tk, p->cache.k, p->cache, p->cache.k_strides, p->heads_k, DR, a.box_rows, kBf16)) ||
+       (rc = make_pool_map(&tv, p->cache.v, p->cache, p->cache.v_strides, p->heads_k, DR, a.box_rows, kBf16))))
+    return rc;
+  if (!launch_with_smem<fmha::paged_few_kernel<D, DR, kBf16, kE4m3, kRows>>(dev, plan.blocks, T::kThreads, T::kSmemBytes,
+                                                                            stream, tq, tk, tv, a))
+    return FMHA_ERR_LAUNCH;
+  return launch_join<kBf16, DR, kRows>(a, plan, p->seqlen_q * a.group, stream);
+}
+
 // (a 32-bit grid of blocks of 256 threads, 8 or 16 of them a row)
 constexpr long long kMaxCacheRows = 1ll << 34;
 
@@ -167,8 +306,9 @@ int fmha_cache_read(const FmhaCacheReadParams* p, void* stream) {
 }
 
 size_t fmha_paged_fwd_workspace_bytes(const FmhaPagedFwdParams* p) {
-  (void)p;
-  return 0;
+  if (p == nullptr || p->batch <= 0 || p->heads_k <= 0 || p->heads_q < p->heads_k || p->seqlen_q <= 0 || p->head_dim <= 0)
+    return 0;
+  return plan_paged(p, sm_count(current_device())).bytes();
 }
 
 int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -186,7 +326,18 @@ int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspac
   if (!aligned16(p->q) || !aligned16(p->o) || !aligned16(workspace)) return FMHA_ERR_BAD_ALIGNMENT;
   if ((rc = check_strides(p->q_strides, p->seqlen_q, p->heads_q, p->batch))) return rc;
   if ((rc = check_strides(p->o_strides, p->seqlen_q, p->heads_q, p->batch))) return rc;
-  (void)workspace_bytes;
+  const int dev = current_device();
+  const PagedPlan plan = plan_paged(p, sm_count(dev));
+  if (plan.bytes() > 0 && (workspace == nullptr || workspace_bytes < plan.bytes())) return FMHA_ERR_WORKSPACE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (plan.kernel_rows > 0) {
+    FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format, {
+      constexpr int D = DR == 64 ? 64 : 128;
+      if (plan.kernel_rows == 16) return launch_few<D, DR, kBf16, kE4m3, 16>(p, plan, workspace, dev, s);
+      if (plan.kernel_rows == 32) return launch_few<D, DR, kBf16, kE4m3, 32>(p, plan, workspace, dev, s);
+      return launch_few<D, DR, kBf16, kE4m3, 64>(p, plan, workspace, dev, s);
+    })
+  }
   fmha::PagedSimpleArgs a;
   a.cache = device_cache(p->cache);
   a.q = static_cast<const uint8_t*>(p->q);
@@ -203,7 +354,6 @@ int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspac
   a.scale = p->scale;
   a.rows = (long long)p->batch * p->seqlen_q * p->heads_q;
   const unsigned grid = (unsigned)((a.rows + 3) / 4);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format,
                       fmha::paged_simple_kernel<DR, kBf16, kE4m3><<<grid, 128, 0, s>>>(a);)
   return cudaGetLastError() == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;

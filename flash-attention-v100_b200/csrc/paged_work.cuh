@@ -1,0 +1,193 @@
+// How attention over the paged cache is cut over the SMs, by lengths that only the device knows.
+//
+// An item is a block of new tokens of one entry with all query heads of one cache head; it has as many KV tiles of
+// 128 keys as its last token sees.  All items' tiles in a row, plus kItemCost tiles for every item's own start and
+// end, are one line of units, which is cut into equal shares: block c of the grid has units [c S, c S + S).  What a
+// block does of one item is a piece.  A piece that is its whole item writes O and LSE; others leave fp32 rows, which
+// paged_join_kernel joins.  So every SM has the same number of keys to read whatever the lengths are, a single long
+// entry is spread over all of them, and an item is cut about as often as there are blocks to an item, no more.
+// Every block works out the line's length and its own place on it from the lengths, a warp at a time.
+#pragma once
+#include "cache_kernels.cuh"
+
+namespace fmha {
+
+struct PagedParams {
+  PagedCache cache;
+  const int32_t *seqused_k, *seqused_q;
+  int batch, heads_k, group, seqlen_q, causal;
+  int blocks_per_entry;   // blocks of new tokens
+  int tokens_per_block;
+  int box_rows;           // rows of a K or V box: what divides both a page and a tile
+  int min_share;          // units a block has at least
+  float scale_log2;       // |scale| * log2(e)
+  int negate;             // scale < 0: the tensor cores form -Q K^T
+  uint16_t* o;
+  long long o_batch, o_row, o_head;  // element strides
+  float* lse;
+  // workspace: rows of pieces (slot, row, DR), their log-sum-exp (slot, row), blocks of every item
+  float *o_part, *lse_part;
+  int2* item_blocks;      // (first block, last block) of an item's tiles
+  int* status;
+};
+
+// Units that an item costs beside its tiles.
+constexpr int kItemCost = 1;
+
+struct PagedPiece {
+  int id;            // item, -1: no more
+  int z, h, token0;  // entry, cache head, first new token
+  int first, tiles;  // KV tiles [first, first + tiles); tiles = 0: the item sees no key at all
+  int slot;          // of its partial rows, -1: the piece is the whole item
+  int sq, sk;        // the entry's lengths
+};
+
+__device__ __forceinline__ void paged_lengths(const PagedParams& p, int z, int& sq, int& sk) {
+  sq = p.seqused_q == nullptr ? p.seqlen_q : max(0, min(p.seqlen_q, __ldg(p.seqused_q + z)));
+  sk = max(0, min(__ldg(p.seqused_k + z), cache_capacity(p.cache)));
+}
+// the last key that token i of an entry sees (-1: none)
+__device__ __forceinline__ int paged_last_key(const PagedParams& p, int i, int sq, int sk) {
+  if (i >= sq) return -1;
+  return p.causal ? max(-1, sk - sq + i) : sk - 1;
+}
+__device__ __forceinline__ int paged_tiles(const PagedParams& p, int token0, int sq, int sk) {
+  if (token0 >= sq) return 0;
+  return (paged_last_key(p, min(token0 + p.tokens_per_block, sq) - 1, sq, sk) + 128) / 128;
+}
+
+// One block's share, walked in order by a converged warp (every lane has the same state).
+struct PagedWork {
+  long long pos, end;      // units still to do
+  long long pair_start;    // first unit of the current (entry, block of tokens), all heads of which follow
+  int pair, tiles;
+  int sq, sk;
+  long long share;
+
+  __device__ __forceinline__ int pair_tiles(const PagedParams& p, int f, int& q, int& k) const {
+    paged_lengths(p, f / p.blocks_per_entry, q, k);
+    return paged_tiles(p, f % p.blocks_per_entry * p.tokens_per_block, q, k);
+  }
+
+  __device__ __forceinline__ void start(const PagedParams& p, int block, int blocks) {
+    const int lane = threadIdx.x & 31;
+    const int pairs = p.batch * p.blocks_per_entry;
+    auto units = [&](int f) -> long long {
+      int q, k;
+      return f < pairs ? (long long)p.heads_k * (pair_tiles(p, f, q, k) + kItemCost) : 0;
+    };
+    long long total = 0;
+    for (int f = lane; f < pairs; f += 32) total += units(f);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    share = max((long long)p.min_share, (total + blocks - 1) / blocks);
+    pos = block * share;
+    end = min(pos + share, total);
+    if (pos >= end) return;
+    long long before = 0;  // units of the pairs before this group of 32
+    for (int f0 = 0;; f0 += 32) {
+      const long long mine = units(f0 + lane);
+      long long sum = mine;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += up;
+      }
+      const uint32_t beyond = __ballot_sync(0xffffffffu, before + sum > pos);
+      if (beyond != 0) {
+        const int l = __ffs(beyond) - 1;
+        pair = f0 + l;
+        pair_start = __shfl_sync(0xffffffffu, before + sum - mine, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    tiles = pair_tiles(p, pair, sq, sk);
+  }
+
+  __device__ __forceinline__ PagedPiece next(const PagedParams& p, int block) {
+    PagedPiece it;
+    it.id = -1;
+    it.tiles = 0;
+    while (pos < end) {
+      const int w = tiles + kItemCost;
+      if (pos - pair_start >= (long long)p.heads_k * w) {
+        pair_start += (long long)p.heads_k * w;
+        ++pair;
+        tiles = pair_tiles(p, pair, sq, sk);
+        continue;
+      }
+      const int h = (int)((pos - pair_start) / w);
+      const long long u0 = pair_start + (long long)h * w;
+      const int first = (int)(pos - u0), last = (int)min((long long)tiles, end - u0);
+      pos = u0 + w;
+      if (first >= tiles && !(tiles == 0 && first == 0)) continue;  // only the item's end: nothing to do for it
+      it.id = pair * p.heads_k + h;
+      it.z = pair / p.blocks_per_entry;
+      it.h = h;
+      it.token0 = pair % p.blocks_per_entry * p.tokens_per_block;
+      it.first = first;
+      it.tiles = last - first;
+      it.slot = first == 0 && last == tiles ? -1 : 2 * block + (first > 0 ? 0 : 1);
+      it.sq = sq;
+      it.sk = sk;
+      if (first == 0 && (threadIdx.x & 31) == 0)
+        p.item_blocks[it.id] = make_int2((int)(u0 / share), tiles > 0 ? (int)((u0 + tiles - 1) / share) : (int)(u0 / share));
+      break;
+    }
+    return it;
+  }
+};
+
+// Joins the pieces of the items that were cut: a warp per row.  Every partial row is normalised by its own row
+// sum; its weight is exp(lse_part - lse).
+template <typename E, int DR, int kRows>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, int rows_per_item, int items, int blocks_of_grid) {
+  grid_dependency_wait();
+  if (p.status != nullptr && *reinterpret_cast<const volatile int*>(p.status) != 0) return;
+  const int lane = threadIdx.x & 31;
+  const long long n = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int item = (int)(n / rows_per_item), row = (int)(n % rows_per_item);
+  if (item >= items) return;
+  const int2 blocks = p.item_blocks[item];
+  // (where a wait ran out and nobody keeps a status word, this may be anything)
+  if (blocks.x < 0 || blocks.x >= blocks.y || blocks.y >= blocks_of_grid) return;
+  const int h = item % p.heads_k, pair = item / p.heads_k;
+  const int z = pair / p.blocks_per_entry;
+  const int token = pair % p.blocks_per_entry * p.tokens_per_block + row / p.group, hq = h * p.group + row % p.group;
+  if (token >= p.seqlen_q) return;
+  auto slot = [&](int b) { return b == blocks.x ? 2 * b + 1 : 2 * b; };
+  // a part that is NaN makes the row NaN
+  float mx = -CUDART_INF_F;
+  for (int b = blocks.x + lane; b <= blocks.y; b += 32) mx = max_nan(mx, p.lse_part[(long long)slot(b) * kRows + row]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+  const float base = mx == -CUDART_INF_F ? 0.f : mx;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  const int col = lane * 4;
+  for (int b = blocks.x; b <= blocks.y; ++b) {
+    const long long at = (long long)slot(b) * kRows + row;
+    const float lp = p.lse_part[at];
+    if (lp == -CUDART_INF_F) continue;  // nothing visible in this piece
+    const float w = lp == base ? 1.f : expf(lp - base);  // (inf - inf would be NaN)
+    sum += w;
+    if (col < DR) {
+      const float4 v = *reinterpret_cast<const float4*>(p.o_part + at * DR + col);
+      acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (lane == 0)
+    p.lse[((long long)z * p.heads_k * p.group + hq) * p.seqlen_q + token] =
+        sum == 0.f ? -CUDART_INF_F : base + logf(sum);
+  if (col < DR) {
+    constexpr bool kBf16 = std::is_same<E, __nv_bfloat16>::value;
+    uint2 v;
+    v.x = pack16x2<kBf16>(acc.x * inv, acc.y * inv);
+    v.y = pack16x2<kBf16>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(p.o + z * p.o_batch + token * p.o_row + hq * p.o_head + col) = v;
+  }
+}
+
+}  // namespace fmha
