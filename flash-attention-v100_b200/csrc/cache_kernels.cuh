@@ -22,14 +22,24 @@ struct PagedCache {
   const int32_t* table;
   long long table_stride;
   int num_pages, page_size, max_pages;
+  // t / page_size for 0 <= t < 2^30 as a product: both are counted in units of 16, so that n < 2^26; with 2^l the power
+  // of two at or above the divisor, m = floor(2^(26 + l) / divisor) + 1 fits 28 bits, and n / divisor is
+  // (n * m) >> (26 + l)
+  unsigned page_mul, page_shift;
 };
+__device__ __forceinline__ int cache_page_index(const PagedCache& c, int t) {
+  return (int)(((unsigned long long)((unsigned)t >> 4) * c.page_mul) >> c.page_shift);
+}
+__device__ __forceinline__ int cache_page_row(const PagedCache& c, int t) {
+  return t - cache_page_index(c, t) * c.page_size;
+}
 
 // tokens an entry can hold at most (fits: checked on the host)
 __device__ __forceinline__ int cache_capacity(const PagedCache& c) { return c.max_pages * c.page_size; }
 
 // the page of token `t` of entry z, -1 where the table names none
 __device__ __forceinline__ int cache_page(const PagedCache& c, int z, int t) {
-  const int page = __ldg(c.table + z * c.table_stride + (unsigned)t / (unsigned)c.page_size);
+  const int page = __ldg(c.table + z * c.table_stride + cache_page_index(c, t));
   return (unsigned)page < (unsigned)c.num_pages ? page : -1;
 }
 
@@ -40,11 +50,15 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
 // 2^-e for e in [-126, 126]
 __device__ __forceinline__ float exp2_neg_int(int e) { return __uint_as_float((uint32_t)(127 - e) << 23); }
 
-// Two codes (low byte first) as fp32
-__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t codes) {
+// Two codes (low byte first) as fp16, exactly, and as fp32
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)codes));
-  return __half22float2(*reinterpret_cast<__half2*>(&h));
+  return h;
+}
+__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t codes) {
+  const uint32_t h = e4m3x2_to_half2(codes);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 // fp32 pair -> codes, rounded to nearest even; a NaN is the code of NaN
 __device__ __forceinline__ uint32_t float2_to_e4m3x2(float lo, float hi) {
@@ -102,7 +116,7 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CacheWriteArgs a
   if (t < 0 || t >= cache_capacity(a.cache)) return;
   const int page = cache_page(a.cache, z, (int)t);
   if (page < 0) return;
-  const int slot = (int)t % a.cache.page_size;
+  const int slot = cache_page_row(a.cache, (int)t);
   const bool in_row = sub * 8 < DR;
   uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
   if (in_row) {
@@ -170,7 +184,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) 
   const int page = t < sk ? cache_page(a.cache, z, t) : -1;
   uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
   if (page >= 0) {
-    const int slot = t % a.cache.page_size;
+    const int slot = cache_page_row(a.cache, t);
     const uint8_t* src[2];
     float s[2];
 #pragma unroll

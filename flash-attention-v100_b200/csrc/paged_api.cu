@@ -39,7 +39,7 @@ int check_cache(const FmhaPagedCache& c, int heads) {
   const bool e4m3 = c.format == FMHA_CACHE_E4M3;
   if (e4m3 && (c.k_scale == nullptr || c.v_scale == nullptr)) return FMHA_ERR_NULL_POINTER;
   if (c.num_pages <= 0 || c.page_size <= 0 || c.page_size % 16 != 0 || c.max_pages <= 0) return FMHA_ERR_BAD_SHAPE;
-  if ((long long)c.max_pages * c.page_size > (1ll << 30)) return FMHA_ERR_TOO_LARGE;
+  if ((long long)c.max_pages * c.page_size >= (1ll << 30)) return FMHA_ERR_TOO_LARGE;
   if (!aligned16(c.k) || !aligned16(c.v)) return FMHA_ERR_BAD_ALIGNMENT;
   int rc;
   const int unit = e4m3 ? 16 : 8;
@@ -58,13 +58,18 @@ fmha::PagedCache device_cache(const FmhaPagedCache& c) {
     return fmha::PagePool{static_cast<uint8_t*>(rows), scales,  s.batch * bytes, s.row * bytes,
                           s.head * bytes,              t.batch, t.row,           t.head};
   };
+  const unsigned unit = (unsigned)c.page_size / 16;
+  unsigned l = 0;
+  while ((1u << l) < unit) ++l;
   return fmha::PagedCache{pool(c.k, c.k_scale, c.k_strides, c.k_scale_strides),
                           pool(c.v, c.v_scale, c.v_strides, c.v_scale_strides),
                           c.block_table,
                           c.block_table_stride,
                           c.num_pages,
                           c.page_size,
-                          c.max_pages};
+                          c.max_pages,
+                          (unsigned)((1ull << (26 + l)) / unit + 1),
+                          26 + l};
 }
 
 // DR, kBf16 and kE4m3 for a kernel of the cache
@@ -100,19 +105,25 @@ fmha::PagedCache device_cache(const FmhaPagedCache& c) {
     FMHA_DISPATCH_CACHE_FORMAT(dtype, format, __VA_ARGS__)             \
   }
 
-// A pool as a 4-D map (D, page_size, H, num_pages), box 64 x box_rows x 1 x 1, 128-byte swizzle, zeros outside
+// A pool as a 4-D map (D, page_size, H, num_pages), 128-byte swizzle, zeros outside; box 64 x box_rows x 1 x 1 of 16-bit
+// elements, 128 x box_rows x 1 x 1 of codes
 int make_pool_map(CUtensorMap* map, const void* base, const FmhaPagedCache& c, const FmhaStrides& s, int heads, int D,
                   int box_rows, bool bf16) {
   EncodeTiledFn encode = get_encode_fn();
   if (encode == nullptr) return FMHA_ERR_NO_DEVICE;
+  const bool codes = c.format == FMHA_CACHE_E4M3;
   // a stride of a size-1 dimension is never used for addressing; make it well-formed
-  const int64_t row = s.row, head = heads > 1 ? s.head : D;
+  const int64_t row = s.row, head = heads > 1 ? s.head : (D + 15) / 16 * 16;
   const int64_t page = c.num_pages > 1 ? s.batch : row * c.page_size;
+  const cuuint64_t unit = codes ? 1 : 2;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)c.page_size, (cuuint64_t)heads, (cuuint64_t)c.num_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const cuuint64_t strides[3] = {(cuuint64_t)row * unit, (cuuint64_t)head * unit, (cuuint64_t)page * unit};
+  const cuuint32_t box[4] = {codes ? 128u : 64u, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map,
+                            codes  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                            : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FMHA_OK : FMHA_ERR_TENSOR_MAP;
@@ -173,6 +184,7 @@ fmha::PagedParams kernel_params(const FmhaPagedFwdParams* p, const PagedPlan& pl
   a.batch = p->batch;
   a.heads_k = p->heads_k;
   a.group = p->heads_q / p->heads_k;
+  a.group_mul = 65536u / a.group + 1;
   a.seqlen_q = p->seqlen_q;
   a.causal = p->causal ? 1 : 0;
   a.blocks_per_entry = plan.blocks_per_entry;
@@ -181,6 +193,10 @@ fmha::PagedParams kernel_params(const FmhaPagedFwdParams* p, const PagedPlan& pl
   a.min_share = plan.min_share;
   a.scale_log2 = std::fabs(p->scale) * 1.4426950408889634f;
   a.negate = p->scale < 0.f;
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.q_batch = p->q_strides.batch;
+  a.q_row = p->q_strides.row;
+  a.q_head = p->q_strides.head;
   a.o = static_cast<uint16_t*>(p->o);
   a.o_batch = p->o_strides.batch;
   a.o_row = p->o_strides.row;
@@ -222,13 +238,12 @@ template <int D, int DR, bool kBf16, bool kE4m3, int kRows>
 int launch_few(const FmhaPagedFwdParams* p, const PagedPlan& plan, void* workspace, int dev, cudaStream_t stream) {
   using T = fmha::FewTraits<D, DR, kBf16, kE4m3, kRows>;
   const fmha::PagedParams a = kernel_params(p, plan, workspace);
-  CUtensorMap tq, tk = {}, tv = {};
+  CUtensorMap tq, tk, tv;
   int rc;
   if ((rc = make_rows_map(&tq, p->q, p->batch, p->seqlen_q, p->heads_q, DR, p->q_strides, a.group, p->seqlen_q, kBf16)))
     return rc;
-  if (!kE4m3 &&
-      ((rc = make_pool_map(&tk, p->cache.k, p->cache, p->cache.k_strides, p->heads_k, DR, a.box_rows, kBf16)) ||
-       (rc = make_pool_map(&tv, p->cache.v, p->cache, p->cache.v_strides, p->heads_k, DR, a.box_rows, kBf16))))
+  if ((rc = make_pool_map(&tk, p->cache.k, p->cache, p->cache.k_strides, p->heads_k, DR, a.box_rows, kBf16)) ||
+      (rc = make_pool_map(&tv, p->cache.v, p->cache, p->cache.v_strides, p->heads_k, DR, a.box_rows, kBf16)))
     return rc;
   if (!launch_with_smem<fmha::paged_few_kernel<D, DR, kBf16, kE4m3, kRows>>(dev, plan.blocks, T::kThreads, T::kSmemBytes,
                                                                             stream, tq, tk, tv, a))
@@ -328,6 +343,9 @@ int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspac
   if ((rc = check_strides(p->o_strides, p->seqlen_q, p->heads_q, p->batch))) return rc;
   const int dev = current_device();
   const PagedPlan plan = plan_paged(p, sm_count(dev));
+  // the line of units (paged_work.cuh) is counted in 32 bits
+  const double tiles = (double)p->cache.max_pages * p->cache.page_size / 128 + 2;
+  if ((double)p->batch * p->heads_k * plan.blocks_per_entry * tiles >= 2147483648.0) return FMHA_ERR_TOO_LARGE;
   if (plan.bytes() > 0 && (workspace == nullptr || workspace_bytes < plan.bytes())) return FMHA_ERR_WORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (plan.kernel_rows > 0) {

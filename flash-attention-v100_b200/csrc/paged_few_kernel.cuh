@@ -12,14 +12,27 @@
 //
 //   warps 0-3   softmax: thread = key; P^T to shared memory; O^T (thread = element of the head) at the end
 //   warp 4      MMA issuer
-//   warp 5      TMA producer of Q
-//   warp 6      source of pieces; 16-bit caches: TMA producer of K and V, a box per page (or per part of one)
-//   warps 8-15  8-bit caches: K and V through registers, codes times scale to 16 bits, into the ring
+//   warp 5      producer of Q
+//   warp 6      source of pieces; TMA producer of K and V, a box per page (or per part of one)
+// 8-bit caches, whose codes and scales arrive in a ring of their own:
+//   warps 8-11  K: codes -> fp16, into tensor memory (a thread has a key there, as in the softmax)
+//   warps 12-15 V: codes times scale -> 16 bits, into the ring that 16-bit caches load directly
 //
-// Shared memory, 128-byte swizzle: ring of K and V tiles (128 x D, boxes of 64 columns), Q (kRows x D, the same
-// boxes), P^T (kRows x 128 keys, two boxes of 64 keys).  Rows of V behind an entry's last token are set to
-// zero before they are multiplied: the page may hold anything there, and 0 * NaN is NaN.
-// Tensor memory: S^T twice, O^T twice, kRows columns each.
+// Shared memory, 128-byte swizzle: ring of K and V tiles (128 x D, boxes of 64 columns; 8-bit caches: of V tiles), Q (kRows
+// x D, the same boxes), P^T (kRows x 128 keys, two boxes of 64 keys), codes (128 rows of 128 bytes).  Rows of V behind
+// an entry's last token are set to zero before they are multiplied: the page may hold anything there, and 0 * NaN is NaN.
+// Tensor memory: S^T twice, O^T twice, kRows columns each; 8-bit caches: K twice, 64 columns each.
+//
+// 8-bit caches are multiplied in fp16, in which a code is exact and a conversion is one instruction for two of them.
+// K goes in without its scale, which the key's softmax thread has as a factor of its scores; Q of bf16 tensors is
+// brought to fp16 under a power of two (see there).  V is multiplied by its scale: exact for exponents of -15 to 7 (a row's
+// largest value between 0.007 and 57344).  Where one of 16 rows has another exponent, bf16 tensors have these rows of V, and
+// P of these keys, in bf16, exactly; fp16 tensors have them rounded to fp16.  The codes come in by TMA, not through
+// registers.
+//
+// The code is kept small: the roles share an instruction cache, and a miss waits in the same queues as HBM's data.
+// With 135 KB of code (everything unrolled, waits among it) warps waited for instructions most of the time, and 64 entries
+// of 2048 to 16384 keys in 8 bits took three times as long as their bytes.
 #pragma once
 #include <cuda.h>
 
@@ -35,19 +48,23 @@ struct FewTraits {
   static constexpr int kQBoxBytes = kRows * 128;
   static constexpr int kQBytes = kBoxes * kQBoxBytes;
   static constexpr int kPBytes = 2 * kRows * 128;
-  static constexpr int kStages = D == 128 ? (kRows == 64 ? 5 : 6) : (kRows == 64 ? 9 : 12);
-  static constexpr int kQBufs = D == 128 && kRows == 64 ? 1 : 2;
-  static constexpr int kItemStages = 4;
+  // ring of K and V (16 bits), or of V alone and of codes (8 bits)
+  static constexpr int kStages = kE4m3 ? (D == 128 ? 3 : 4) : D == 128 ? (kRows == 16 ? 6 : 5) : (kRows == 64 ? 9 : 12);
+  static constexpr int kCodeStages = !kE4m3 ? 0 : D == 128 && kRows == 64 ? 4 : 6;
+  static constexpr int kCodeBytes = 128 * 128;
+  static constexpr int kQBufs = D == 128 && (kRows == 64 || (kE4m3 && kRows == 32)) ? 1 : 2;
+  static constexpr int kItemStages = 8;
   static constexpr int kThreads = kE4m3 ? 512 : 224;
-  static constexpr int kSmemBytes = 1024 + kStages * kTileBytes + kQBufs * kQBytes + 2 * kPBytes;
-  static constexpr int kTmemCols = 4 * kRows;
-  static constexpr uint32_t kIdescQK = umma_idesc_f16(128, kRows, 0, 0, kBf16);
-  static constexpr uint32_t kIdescPV = umma_idesc_f16(128, kRows, 1, 0, kBf16);
+  static constexpr int kSmemBytes =
+      1024 + kStages * kTileBytes + kCodeStages * kCodeBytes + kQBufs * kQBytes + 2 * kPBytes;
+  static constexpr int kTmemCols = !kE4m3 ? 4 * kRows : kRows == 64 ? 512 : 256;
+  // 8-bit caches are multiplied in fp16 (see the converting warps)
+  static constexpr uint32_t kIdescQK = umma_idesc_f16(128, kRows, 0, 0, kBf16 && !kE4m3);
+  static constexpr uint32_t kIdescPV = umma_idesc_f16(128, kRows, 1, 0, kBf16 && !kE4m3);
+  static constexpr uint32_t kIdescPVBf16 = umma_idesc_f16(128, kRows, 1, 0, true);
   // V^T has D rows; with D = 64 the upper 64 of the 128 repeat the lower ones, unused
   static constexpr uint32_t kLboV = D == 128 ? kBoxBytes : 0;
-  // 16-byte chunks of a row of codes, and how many of a tile's a converting thread has
-  static constexpr int kChunks = DR / 16;
-  static constexpr int kPerThread = 128 * kChunks / 256;
+  static constexpr int kChunks = DR / 16;  // 16-byte chunks of a row of codes
 };
 
 __device__ __forceinline__ bool vote_any(uint32_t id, uint32_t count, bool mine) {
@@ -107,9 +124,20 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   __shared__ uint64_t bar_q_full[2], bar_q_free[2], bar_s_full[2], bar_s_free[2], bar_p_full[2], bar_p_free[2],
       bar_o_full[2], bar_o_free[2];
   __shared__ float warp_part[4][kRows];   // per warp: a row's maximum, or its sum
-  __shared__ __align__(16) float row_neg[kRows];    // -m * c, 0 where there is no finite reference
+  __shared__ __align__(16) float row_neg[kRows];    // minus the reference, 0 where there is no finite one
   __shared__ __align__(16) float row_scale[kRows];  // what O is multiplied by
   __shared__ __align__(16) int row_last[kRows];     // last key a row sees
+  __shared__ long long row_out[kRows];              // where a row of O lies, from its block's first row on
+  // 8-bit caches: codes and scale bytes of a stage; K in tensor memory, and its scale bytes (a tile's are read after the
+  // next two may have been converted); whether 16 rows of V in a slot are bf16; the power of two that a piece's Q was divided
+  // by (Q is three pieces ahead at most)
+  __shared__ uint64_t bar_code_full[kE4m3 ? T::kCodeStages : 1], bar_code_empty[kE4m3 ? T::kCodeStages : 1];
+  __shared__ uint64_t bar_kt_full[2], bar_kt_free[2];
+  __shared__ uint32_t code_scale[kE4m3 ? T::kCodeStages : 1][128];  // the aligned word around a row's byte
+  __shared__ uint8_t code_select[kE4m3 ? T::kCodeStages : 1][32];    // which byte of it, two bits for each of four rows
+  __shared__ uint8_t k_scale[kE4m3 ? 4 : 1][128];
+  __shared__ __align__(8) uint8_t v_bf16[kE4m3 ? kStages : 1][8];
+  __shared__ float q_scale[4];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_word;
   __shared__ int skip_cta;
@@ -127,15 +155,22 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   const uint32_t ring_smem = smem_base;
   const uint32_t q_smem = ring_smem + kStages * T::kTileBytes;
   const uint32_t p_smem = q_smem + T::kQBufs * T::kQBytes;
+  [[maybe_unused]] const uint32_t code_smem = p_smem + 2 * T::kPBytes;
+  // position of V of tile n in the ring
+  auto v_at = [](uint32_t n) { return kE4m3 ? n : 2 * n + 1; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < T::kItemStages; ++s) {
       mbar_init(smem_u32(&bar_item_full[s]), 1);
-      mbar_init(smem_u32(&bar_item_empty[s]), kE4m3 ? 14 : 6);  // MMA, Q, four softmax (and eight converting) warps
+      mbar_init(smem_u32(&bar_item_empty[s]), kE4m3 ? 14 : 6);  // MMA, Q, four softmax (eight converting) warps
     }
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&bar_kv_full[s]), kE4m3 ? 8 : 1);
+      mbar_init(smem_u32(&bar_kv_full[s]), kE4m3 ? 4 : 1);
       mbar_init(smem_u32(&bar_kv_empty[s]), 1);
+    }
+    for (int s = 0; s < T::kCodeStages; ++s) {
+      mbar_init(smem_u32(&bar_code_full[s]), 33);  // TMA's thread, a warp's copies of scales
+      mbar_init(smem_u32(&bar_code_empty[s]), 4);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&bar_q_full[b]), 1);
@@ -146,6 +181,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       mbar_init(smem_u32(&bar_p_free[b]), 1);
       mbar_init(smem_u32(&bar_o_full[b]), 1);
       mbar_init(smem_u32(&bar_o_free[b]), 4);
+      mbar_init(smem_u32(&bar_kt_full[b]), 4);
+      mbar_init(smem_u32(&bar_kt_free[b]), 1);
     }
     fence_barrier_init();
   }
@@ -155,6 +192,10 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   }
   // rows of Q that no load fills stay zero: their scores are 0
   for (uint32_t at = threadIdx.x * 16; at < T::kQBufs * T::kQBytes; at += blockDim.x * 16) sts128(q_smem + at, 0, 0, 0, 0);
+  if (threadIdx.x < kRows) {
+    const int t = row_token(p, threadIdx.x);
+    row_out[threadIdx.x] = t * p.o_row + ((int)threadIdx.x - t * p.group) * p.o_head;
+  }
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
@@ -165,7 +206,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   auto take_item = [&]() -> PagedPiece {
     const uint32_t s = item_cnt % T::kItemStages;
     PagedPiece it;
-    if (mbar_wait_warp(smem_u32(&bar_item_full[s]), (item_cnt / T::kItemStages) & 1, &abort_word, 1)) {
+    if (rolled_wait_warp(smem_u32(&bar_item_full[s]), (item_cnt / T::kItemStages) & 1, &abort_word, 1)) {
       it = items[s];
       it.id = __shfl_sync(0xffffffffu, it.id, 0);
       it.tiles = __shfl_sync(0xffffffffu, it.tiles, 0);
@@ -179,17 +220,28 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     return it;
   };
 
+  // the scale byte of a row in a stage of codes
+  [[maybe_unused]] auto scale_byte = [&](uint32_t stage, int row) -> uint32_t {
+    return code_scale[stage][row] >> ((code_select[stage][row >> 2] >> (row % 4 * 2) & 3) * 8) & 0xffu;
+  };
+
   if (warp == 6) {
     // =========================== source of pieces, K and V producer ===========================
+    // a lane per box: 128 / box_rows parts of a tile, kBoxes column blocks of each (codes: one)
+    constexpr int kCols = kE4m3 ? 1 : T::kBoxes;
+    constexpr uint32_t kRing = kE4m3 ? T::kCodeStages : kStages;
+    constexpr uint32_t kBytes = kE4m3 ? T::kCodeBytes : T::kTileBytes;
+    const int sub = lane / kCols, box = lane % kCols;
+    const bool mine = sub < 128 / p.box_rows;
+    const uint32_t dst = (kE4m3 ? code_smem : ring_smem) + box * T::kBoxBytes + sub * p.box_rows * 128;
     PagedWork work;
     work.start(p, blockIdx.x, gridDim.x);
     bool ok = true;
-    uint32_t published = 0, loaded = 0;
-    [[maybe_unused]] const int subs = 128 / p.box_rows;
+    uint32_t slot = 0, phase = 1, published = 0;
     while (ok) {
       const PagedPiece it = work.next(p, blockIdx.x);
       const uint32_t s = published % T::kItemStages, round = published / T::kItemStages;
-      if (round > 0 && !mbar_wait_warp(smem_u32(&bar_item_empty[s]), (round - 1) & 1, &abort_word, 2)) break;
+      if (round > 0 && !rolled_wait_warp(smem_u32(&bar_item_empty[s]), (round - 1) & 1, &abort_word, 2)) break;
       if (lane == 0) {
         items[s] = it;
         mbar_arrive(smem_u32(&bar_item_full[s]));
@@ -197,37 +249,55 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       __syncwarp();
       ++published;
       if (it.id < 0) break;
-      if constexpr (!kE4m3) {
-        // a lane per box: 128 / box_rows parts of the tile, kBoxes column blocks of each
-        const int sub = lane / T::kBoxes, box = lane % T::kBoxes;
-        const bool mine = sub < subs;
-        const uint32_t dst = box * T::kBoxBytes + sub * p.box_rows * 128;
-        auto place = [&](int tile, int& row) {  // page of this lane's part (num_pages, outside the pool: zeros)
-          const int key = (it.first + tile) * 128 + sub * p.box_rows;
-          row = key % p.cache.page_size;
-          if (!mine || key >= it.sk) return p.cache.num_pages;
-          const int page = cache_page(p.cache, it.z, key);
-          return page < 0 ? p.cache.num_pages : page;
-        };
-        int row, page = place(0, row);
+      auto place = [&](int tile, int& row) {  // page of this lane's part (num_pages, outside the pool: zeros)
+        const int key = (it.first + tile) * 128 + sub * p.box_rows;
+        row = cache_page_row(p.cache, key);
+        if (!mine || key >= it.sk) return p.cache.num_pages;
+        const int page = cache_page(p.cache, it.z, key);
+        return page < 0 ? p.cache.num_pages : page;
+      };
+      int row_next = 0, page_next = 0;
 #pragma unroll 1
-        for (int j = 0; ok && j < it.tiles; ++j) {
-          int row_next = 0, page_next = 0;
-          if (j + 1 < it.tiles) page_next = place(j + 1, row_next);
+      for (int j = -1; ok && j < it.tiles; ++j) {
+        const int row = row_next, page = page_next;
+        if (j + 1 < it.tiles) page_next = place(j + 1, row_next);
+        if (j < 0) continue;
 #pragma unroll 1
-          for (int n = 0; n < 2; ++n) {
-            const uint32_t slot = loaded % kStages;
-            if (!(ok = mbar_wait_warp(smem_u32(&bar_kv_empty[slot]), (loaded / kStages & 1) ^ 1, &abort_word, 3))) break;
-            if (lane == 0) mbar_arrive_expect_tx(smem_u32(&bar_kv_full[slot]), T::kTileBytes);
+        for (int n = 0; n < 2; ++n) {
+          uint64_t* const full = kE4m3 ? &bar_code_full[slot] : &bar_kv_full[slot];
+          uint64_t* const empty = kE4m3 ? &bar_code_empty[slot] : &bar_kv_empty[slot];
+          if (!(ok = rolled_wait_warp(smem_u32(empty), phase, &abort_word, 3))) break;
+          if constexpr (kE4m3) {
+            // scales: four rows a lane, in one page; the copy is of words, each the one that a row's byte is in (a
+            // word that holds a byte of an allocation is in it)
+            const int from = lane * 4 / p.box_rows, page4 = __shfl_sync(0xffffffffu, page, from);
+            const long long row4 = __shfl_sync(0xffffffffu, row, from) + lane * 4 % p.box_rows;
+            const PagePool& pool = n ? p.cache.v : p.cache.k;
+            const uint8_t* src = pool.scales + page4 * pool.scale_page + row4 * pool.scale_row + it.h * pool.scale_head;
+            const uint32_t to = smem_u32(&code_scale[slot][lane * 4]);
+            uint32_t select = 0;
+            if (page4 < p.cache.num_pages) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i, src += pool.scale_row) {
+                const size_t at = reinterpret_cast<size_t>(src);
+                copy_async4(to + 4 * i, reinterpret_cast<const void*>(at & ~size_t(3)));
+                select |= (uint32_t)(at & 3) << (2 * i);
+              }
+            } else {
+              sts128(to, 127, 127, 127, 127);
+            }
+            code_select[slot][lane] = (uint8_t)select;
+            copy_async_arrive(smem_u32(full));
             __syncwarp();
-            if (mine)
-              tma_load_4d(ring_smem + slot * T::kTileBytes + dst, n ? &tm_v : &tm_k, smem_u32(&bar_kv_full[slot]), box * 64,
-                          row, it.h, page);
-            __syncwarp();
-            ++loaded;
           }
-          row = row_next;
-          page = page_next;
+          if (lane == 0) mbar_arrive_expect_tx(smem_u32(full), kBytes);
+          __syncwarp();
+          if (mine) tma_load_4d(dst + slot * kBytes, n ? &tm_v : &tm_k, smem_u32(full), box * 64, row, it.h, page);
+          __syncwarp();
+          if (++slot == kRing) {
+            slot = 0;
+            phase ^= 1;
+          }
         }
       }
     }
@@ -240,8 +310,42 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       if (it.id < 0) break;
       if (it.tiles == 0) continue;
       const uint32_t b = used % T::kQBufs, round = used / T::kQBufs;
-      if (round > 0 && !mbar_wait_warp(smem_u32(&bar_q_free[b]), (round - 1) & 1, &abort_word, 4)) break;
-      if (elect_one()) {
+      if (round > 0 && !rolled_wait_warp(smem_u32(&bar_q_free[b]), (round - 1) & 1, &abort_word, 4)) break;
+      if constexpr (kE4m3 && kBf16) {
+        // Q in fp16, like K: divided by the power of two that brings its largest value to [2^14, 2^15).  What is less
+        // than 2^-28 of that value loses bits, nothing is off by more than 2^-39 of it.
+        const int total = p.seqlen_q * p.group * (DR / 8);  // chunks of 8 elements
+        const uint16_t* src = p.q + it.z * p.q_batch + it.token0 * p.q_row + it.h * p.group * p.q_head;
+        auto chunk_of = [&](int n) {
+          const int r = n / (DR / 8), t = row_token(p, r);
+          return __ldg(reinterpret_cast<const uint4*>(src + t * p.q_row + (r - t * p.group) * p.q_head) + n % (DR / 8));
+        };
+        uint32_t top = 0;  // exponent fields of finite values
+#pragma unroll 1
+        for (int n = lane; n < total; n += 32) {
+          const uint4 x = chunk_of(n);
+          for (uint32_t w : {x.x, x.y, x.z, x.w})
+            for (uint32_t ex : {w >> 7 & 0xffu, w >> 23 & 0xffu}) top = ex == 255 ? top : max(top, ex);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const int e = top == 0 ? 0 : (int)top - 127 - 14;  // (-140 to 113)
+        // 2^-e in two factors: one alone need not be a normal number
+        const float s0 = __uint_as_float((uint32_t)(127 - e / 2) << 23), s1 = __uint_as_float((uint32_t)(127 - (e - e / 2)) << 23);
+#pragma unroll 1
+        for (int n = lane; n < total; n += 32) {
+          float f[8];
+          unpack8<__nv_bfloat16>(chunk_of(n), f);
+          const int r = n / (DR / 8), c = n % (DR / 8);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * s0 * s1;
+          sts128(q_smem + b * T::kQBytes + (c >> 3) * T::kQBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), pack_half2(f[0], f[1]),
+                 pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+        }
+        if (lane == 0) q_scale[used & 3] = __uint_as_float(e < -126 ? 1u << (149 + e) : (uint32_t)(127 + e) << 23);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_q_full[b]));
+      } else if (elect_one()) {
         const uint32_t bar = smem_u32(&bar_q_full[b]);
         mbar_arrive_expect_tx(bar, bytes);
 #pragma unroll
@@ -252,33 +356,43 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       ++used;
     }
   } else if (warp == 4) {
-    // =========================== MMA issuer (converged warp, elected issue) ===================
+    // =========================== MMA issuer ===================
     // S^T of a tile is issued before O^T of the one before it, so that the tensor pipe has work while the softmax
     // warps have the tile.  K of tile n is slot 2n of the ring, V slot 2n + 1.
-    const uint32_t idesc_qk = T::kIdescQK | (p.negate ? kIdescNegateA : 0u);
     uint32_t n = 0, piece = 0;
     bool ok = true;
     bool pending = false, pending_first = false, pending_last = false;
     uint32_t pending_piece = 0;
     auto issue_pv = [&]() {
-      const uint32_t m = n - 1, b = m & 1, at = 2 * m + 1, slot = at % kStages;
-      ok = mbar_wait_warp(smem_u32(&bar_p_full[b]), (m >> 1) & 1, &abort_word, 5) &&
-           mbar_wait_warp(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 6);
+      const uint32_t m = n - 1, b = m & 1, at = v_at(m), slot = at % kStages;
+      ok = rolled_wait_warp(smem_u32(&bar_p_full[b]), (m >> 1) & 1, &abort_word, 5) &&
+           rolled_wait_warp(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 6);
       const uint32_t ob = pending_piece & 1;
       if (ok && pending_first && pending_piece >= 2)
-        ok = mbar_wait_warp(smem_u32(&bar_o_free[ob]), ((pending_piece >> 1) - 1) & 1, &abort_word, 7);
+        ok = rolled_wait_warp(smem_u32(&bar_o_free[ob]), ((pending_piece >> 1) - 1) & 1, &abort_word, 7);
       if (!ok) return;
       tc_fence_after();
       const uint32_t a_lo = umma_desc_lo(ring_smem + slot * T::kTileBytes, T::kLboV);
       const uint32_t b_lo = umma_desc_lo(p_smem + b * T::kPBytes, kLboKMajor);
+      uint2 in_bf16 = make_uint2(0, 0);  // a byte for each 16 keys
+      if constexpr (kE4m3 && kBf16) {
+        in_bf16 = *reinterpret_cast<const uint2*>(v_bf16[slot]);
+        in_bf16.x = __shfl_sync(0xffffffffu, in_bf16.x, 0);
+        in_bf16.y = __shfl_sync(0xffffffffu, in_bf16.y, 0);
+      }
+      if (elect_one()) {
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks)
-        umma_ss_elect(tmem_base + (2 + ob) * kRows, a_lo + ((ks * 2048) >> 4),
-                      b_lo + (((ks >> 2) * kRows * 128 + (ks & 3) * 32) >> 4), T::kIdescPV,
-                      (!pending_first || ks > 0) ? 1u : 0u);
-      umma_commit_elect(smem_u32(&bar_kv_empty[slot]));
-      umma_commit_elect(smem_u32(&bar_p_free[b]));
-      if (pending_last) umma_commit_elect(smem_u32(&bar_o_full[ob]));
+        for (int ks = 0; ks < 8; ++ks) {
+          const bool bf = ((ks < 4 ? in_bf16.x : in_bf16.y) >> (ks % 4 * 8) & 1) != 0;
+          umma_ss(tmem_base + (2 + ob) * kRows, a_lo + ((ks * 2048) >> 4),
+                  b_lo + (((ks >> 2) * kRows * 128 + (ks & 3) * 32) >> 4), bf ? T::kIdescPVBf16 : T::kIdescPV,
+                  (!pending_first || ks > 0) ? 1u : 0u);
+        }
+        umma_commit(smem_u32(&bar_kv_empty[slot]));
+        umma_commit(smem_u32(&bar_p_free[b]));
+        if (pending_last) umma_commit(smem_u32(&bar_o_full[ob]));
+      }
+      __syncwarp();
       pending = false;
     };
     while (ok) {
@@ -287,20 +401,31 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
 #pragma unroll 1
       for (int j = 0; j < it.tiles; ++j) {
         const uint32_t b = n & 1, at = 2 * n, slot = at % kStages, qb = piece % T::kQBufs;
-        if (j == 0) ok = mbar_wait_warp(smem_u32(&bar_q_full[qb]), piece / T::kQBufs & 1, &abort_word, 8);
-        ok = ok && mbar_wait_warp(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 9);
-        if (ok && n >= 2) ok = mbar_wait_warp(smem_u32(&bar_s_free[b]), ((n >> 1) - 1) & 1, &abort_word, 10);
+        if (j == 0) ok = rolled_wait_warp(smem_u32(&bar_q_full[qb]), piece / T::kQBufs & 1, &abort_word, 8);
+        if (kE4m3)
+          ok = ok && rolled_wait_warp(smem_u32(&bar_kt_full[b]), (n >> 1) & 1, &abort_word, 18);
+        else
+          ok = ok && rolled_wait_warp(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 9);
+        if (ok && n >= 2) ok = rolled_wait_warp(smem_u32(&bar_s_free[b]), ((n >> 1) - 1) & 1, &abort_word, 10);
         if (!ok) break;
         tc_fence_after();
         const uint32_t a_lo = umma_desc_lo(ring_smem + slot * T::kTileBytes, kLboKMajor);
         const uint32_t b_lo = umma_desc_lo(q_smem + qb * T::kQBytes, kLboKMajor);
+        if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < DR / 16; ++ks)
-          umma_ss_elect(tmem_base + b * kRows, a_lo + (((ks >> 2) * T::kBoxBytes + (ks & 3) * 32) >> 4),
-                        b_lo + (((ks >> 2) * T::kQBoxBytes + (ks & 3) * 32) >> 4), idesc_qk, ks > 0 ? 1u : 0u);
-        umma_commit_elect(smem_u32(&bar_kv_empty[slot]));
-        umma_commit_elect(smem_u32(&bar_s_full[b]));
-        if (j == it.tiles - 1) umma_commit_elect(smem_u32(&bar_q_free[qb]));
+          for (int ks = 0; ks < DR / 16; ++ks) {
+            const uint32_t q_lo = b_lo + (((ks >> 2) * T::kQBoxBytes + (ks & 3) * 32) >> 4);
+            if (kE4m3)
+              umma_ts(tmem_base + b * kRows, tmem_base + 4 * kRows + b * 64 + ks * 8, q_lo, T::kIdescQK, ks > 0 ? 1u : 0u);
+            else
+              umma_ss(tmem_base + b * kRows, a_lo + (((ks >> 2) * T::kBoxBytes + (ks & 3) * 32) >> 4), q_lo, T::kIdescQK,
+                      ks > 0 ? 1u : 0u);
+          }
+          umma_commit(smem_u32(kE4m3 ? &bar_kt_free[b] : &bar_kv_empty[slot]));
+          umma_commit(smem_u32(&bar_s_full[b]));
+          if (j == it.tiles - 1) umma_commit(smem_u32(&bar_q_free[qb]));
+        }
+        __syncwarp();
         if (pending) issue_pv();
         if (!ok) break;
         ++n;
@@ -316,26 +441,26 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     // =========================== softmax, O ===========================
     const int tid = threadIdx.x;  // key of the tile, element of the head
     const uint32_t lane_addr = uint32_t(warp * 32) << 16;
-    const float c = p.scale_log2;
     const int rows = p.seqlen_q * p.group;
     // P^T: row r at r * 128 bytes, keys 64 and up in a second box, 16-byte chunks swizzled by the row
     const uint32_t p_key = (tid >> 6) * (kRows * 128) + (tid & 7) * 2;
     const uint32_t p_chunk = (tid >> 3) & 7;
-    float ref = -CUDART_INF_F;  // (threads below kRows) reference of row tid
+    float ref = -CUDART_INF_F;  // (threads below kRows) reference of row tid: a score times log2(e)
     uint32_t n = 0, piece = 0;
     for (;;) {
       const PagedPiece it = take_item();
       if (it.id < 0) break;
-      const int token_of_row = tid / p.group;
+      const int token_of_row = row_token(p, tid);
       const bool row_here = tid < kRows && tid < rows;
-      const int my_token = it.token0 + token_of_row, my_head = it.h * p.group + tid % p.group;
+      const int my_token = it.token0 + token_of_row, my_head = it.h * p.group + tid - token_of_row * p.group;
       float* const my_lse = it.slot >= 0 ? p.lse_part + (long long)it.slot * kRows + tid
                                          : p.lse + ((long long)it.z * p.heads_k * p.group + my_head) * p.seqlen_q + my_token;
       if (it.tiles == 0) {  // nobody sees anything: O = 0, LSE = -inf
         if (row_here) *my_lse = -CUDART_INF_F;
         if (tid < DR)
+#pragma unroll 1
           for (int r = 0; r < rows; ++r)
-            p.o[it.z * p.o_batch + (it.token0 + r / p.group) * p.o_row + (it.h * p.group + r % p.group) * p.o_head + tid] = 0;
+            p.o[it.z * p.o_batch + it.token0 * p.o_row + it.h * p.group * p.o_head + row_out[r] + tid] = 0;
         continue;
       }
       // rows that do not exist have scores of 0 and see every key there is
@@ -353,8 +478,13 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         const uint32_t b = n & 1;
         const int key0 = (it.first + j) * 128, key = key0 + tid;
         const uint32_t tS = tmem_base + lane_addr + b * kRows, tO = tmem_base + lane_addr + (2 + (piece & 1)) * kRows;
-        mbar_wait(smem_u32(&bar_s_full[b]), (n >> 1) & 1, &abort_word, 11);
+        rolled_wait(smem_u32(&bar_s_full[b]), (n >> 1) & 1, &abort_word, 11);
         tc_fence_after();
+        float c = p.negate ? -p.scale_log2 : p.scale_log2;
+        if constexpr (kE4m3) {
+          if (kBf16) c *= q_scale[piece & 3];
+          c *= scale_value(k_scale[n & 3][tid]);
+        }
         if (j > 0) {
           // would an exponential be too large?  (2^10: P has to stay far from the 65504 of fp16)
           float top = -CUDART_INF_F;
@@ -384,7 +514,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             if (r0 == 0 && j == 0) named_bar_sync(1, 128);  // row_last is there
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float m = warp_max(key <= row_last[r0 + i] ? __uint_as_float(s[i]) : -CUDART_INF_F);
+              const float m = warp_max(key <= row_last[r0 + i] ? __uint_as_float(s[i]) * c : -CUDART_INF_F);
               mine = lane == i ? m : mine;
             }
             if (lane < 16) warp_part[warp][r0 + lane] = mine;
@@ -394,15 +524,15 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           if (tid < kRows) {
             const float m = fmaxf(fmaxf(fmaxf(warp_part[0][tid], warp_part[1][tid]),
                                         fmaxf(warp_part[2][tid], warp_part[3][tid])), ref);
-            row_scale[tid] = isinf(m) || isinf(ref) ? 1.f : fast_exp2((ref - m) * c);
-            row_neg[tid] = isinf(m) ? 0.f : -m * c;
+            row_scale[tid] = isinf(m) || isinf(ref) ? 1.f : fast_exp2(ref - m);
+            row_neg[tid] = isinf(m) ? 0.f : -m;
             ref = m;
             unset = m == -CUDART_INF_F && row_last[tid] > key0 + 127;
           }
           force = vote_any(1, 128, unset);
           if (j > 0) {
             // O^T of the tiles before is complete
-            mbar_wait(smem_u32(&bar_p_free[b ^ 1]), ((n - 1) >> 1) & 1, &abort_word, 12);
+            rolled_wait(smem_u32(&bar_p_free[b ^ 1]), ((n - 1) >> 1) & 1, &abort_word, 12);
             tc_fence_after();
 #pragma unroll
             for (int r0 = 0; r0 < kRows; r0 += 16) {
@@ -422,8 +552,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         }
         if (!kE4m3 && key0 + 128 > it.sk) {
           // rows of V behind the entry's end
-          const uint32_t at = 2 * n + 1, slot = at % kStages;
-          mbar_wait(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 13);
+          const uint32_t at = v_at(n), slot = at % kStages;
+          rolled_wait(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 13);
           if (key >= it.sk) {
 #pragma unroll
             for (int box = 0; box < T::kBoxes; ++box)
@@ -432,7 +562,13 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
                 sts128(ring_smem + slot * T::kTileBytes + box * T::kBoxBytes + tid * 128 + i * 16, 0, 0, 0, 0);
           }
         }
-        if (n >= 2) mbar_wait(smem_u32(&bar_p_free[b]), ((n >> 1) - 1) & 1, &abort_word, 14);
+        [[maybe_unused]] bool bf = false;
+        if constexpr (kE4m3 && kBf16) {
+          const uint32_t at = v_at(n), slot = at % kStages;
+          rolled_wait(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 17);
+          bf = v_bf16[slot][tid >> 4] != 0;
+        }
+        if (n >= 2) rolled_wait(smem_u32(&bar_p_free[b]), ((n >> 1) - 1) & 1, &abort_word, 14);
         const uint32_t dst = p_smem + b * T::kPBytes + p_key;
 #pragma unroll
         for (int r0 = 0; r0 < kRows; r0 += 16) {
@@ -455,7 +591,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             for (int u = 0; u < 4; u += 2) {
               l[r0 + i + u] += e[u];
               l[r0 + i + u + 1] += e[u + 1];
-              const uint32_t w = pack16x2<kBf16>(e[u], e[u + 1]);
+              uint32_t w = pack16x2<kBf16 && !kE4m3>(e[u], e[u + 1]);
+              if (kE4m3 && kBf16 && bf) w = pack_bf16x2(e[u], e[u + 1]);
               const int r = r0 + i + u;
               sts16(dst + r * 128 + ((p_chunk ^ (r & 7)) << 4), w);
               sts16(dst + (r + 1) * 128 + ((p_chunk ^ ((r + 1) & 7)) << 4), w >> 16);
@@ -483,11 +620,11 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       if (tid < kRows) {
         const float sum = (warp_part[0][tid] + warp_part[1][tid]) + (warp_part[2][tid] + warp_part[3][tid]);
         row_scale[tid] = sum == 0.f ? 0.f : 1.f / sum;
-        if (row_here) *my_lse = sum == 0.f ? -CUDART_INF_F : (ref * c + log2f(sum)) * 0.6931471805599453f;
+        if (row_here) *my_lse = sum == 0.f ? -CUDART_INF_F : (ref + log2f(sum)) * 0.6931471805599453f;
       }
       named_bar_sync(1, 128);
       const uint32_t ob = piece & 1;
-      mbar_wait(smem_u32(&bar_o_full[ob]), (piece >> 1) & 1, &abort_word, 15);
+      rolled_wait(smem_u32(&bar_o_full[ob]), (piece >> 1) & 1, &abort_word, 15);
       tc_fence_after();
       uint16_t* const out = p.o + it.z * p.o_batch + it.token0 * p.o_row + it.h * p.group * p.o_head + tid;
       float* const part = p.o_part + (long long)it.slot * kRows * DR + tid;
@@ -502,11 +639,11 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             const int r = r0 + i;
             if (r >= rows) break;
             // (a row without a visible key: P was 0, but 0 times what V holds need not be)
-            const float v = row_scale[r] == 0.f ? 0.f : __uint_as_float(o[i]) * row_scale[r];
+            const float a = row_scale[r], v = a == 0.f ? 0.f : __uint_as_float(o[i]) * a;
             if (it.slot >= 0)
               part[r * DR] = v;
             else
-              out[r / p.group * p.o_row + r % p.group * p.o_head] = (uint16_t)pack16x2<kBf16>(v, 0.f);
+              out[row_out[r]] = (uint16_t)pack16x2<kBf16>(v, 0.f);
           }
         }
       }
@@ -515,86 +652,110 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       if (lane == 0) mbar_arrive(smem_u32(&bar_o_free[ob]));
       ++piece;
     }
-  } else if (kE4m3 && warp >= 8) {
-    // =========================== 8-bit K and V into the ring ===========================
-    // A thread has the same chunks (row, 16 codes) of every tile.  Two tiles are in flight in registers, 64 KB per SM,
-    // while a third is converted.
-    constexpr int kPer = T::kPerThread, kDepth = 2;
-    const int t = threadIdx.x - 256;
-    struct Chunk {
-      uint4 codes[2][kPer];
-      uint32_t scale[2][kPer];
-    };
-    Chunk buf[kDepth];
-    PagedPiece it;
-    it.id = 0;
-    it.tiles = 0;
-    int j = 0;
-    // the next tile of this block's pieces -> registers; false: there is none
-    auto fetch = [&](Chunk& x) -> bool {
-      while (j >= it.tiles) {
-        if (it.id < 0) return false;
-        it = take_item();
-        j = 0;
-      }
+  } else if constexpr (kE4m3) {
+    if (warp >= 8 && warp < 12) {
+      // =========================== K: codes -> fp16 in tensor memory, thread = key ===========================
+      const int tid = threadIdx.x - 256;
+      const uint32_t tK = tmem_base + (uint32_t(tid & ~31) << 16) + 4 * kRows;
+      uint32_t n = 0;
+      bool ok = true;
+      while (ok) {
+        const PagedPiece it = take_item();
+        if (it.id < 0) break;
+  #pragma unroll 1
+        for (int j = 0; j < it.tiles; ++j, ++n) {
+          const uint32_t b = n & 1, at = 2 * n, slot = at % T::kCodeStages;
+          ok = rolled_wait_warp(smem_u32(&bar_code_full[slot]), at / T::kCodeStages & 1, &abort_word, 20);
+          if (ok && n >= 2) ok = rolled_wait_warp(smem_u32(&bar_kt_free[b]), ((n >> 1) - 1) & 1, &abort_word, 21);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t src = code_smem + slot * T::kCodeBytes + tid * 128;
+          k_scale[n & 3][tid] = (uint8_t)scale_byte(slot, tid);
+  #pragma unroll 1
+          for (int i = 0; i < T::kChunks; i += 2) {  // 32 elements, 16 columns of tensor memory
+            uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int idx = t + 256 * i, row = idx / T::kChunks, chunk = idx % T::kChunks;
-        const int key = (it.first + j) * 128 + row;
-        const int page = key < it.sk ? cache_page(p.cache, it.z, key) : -1;
-        const int slot = key % p.cache.page_size;
+            for (int half = 0; half < 2; ++half) {
+              const float4 f = lds128(src + (((i + half) ^ (tid & 7)) << 4));
+              const uint32_t codes[4] = {__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w)};
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const PagePool& pool = n ? p.cache.v : p.cache.k;
-          x.codes[n][i] = make_uint4(0, 0, 0, 0);
-          x.scale[n][i] = 127;
-          if (page >= 0) {
-            x.codes[n][i] = __ldg(reinterpret_cast<const uint4*>(pool.rows + page * pool.page + slot * pool.row + it.h * pool.head) + chunk);
-            x.scale[n][i] = __ldg(pool.scales + page * pool.scale_page + slot * pool.scale_row + it.h * pool.scale_head);
+              for (int u = 0; u < 4; ++u) {
+                w[half * 8 + 2 * u] = e4m3x2_to_half2(codes[u] & 0xffffu);
+                w[half * 8 + 2 * u + 1] = e4m3x2_to_half2(codes[u] >> 16);
+              }
+            }
+            tmem_st16(tK + b * 64 + i * 8, w);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(smem_u32(&bar_kt_full[b]));
+            mbar_arrive(smem_u32(&bar_code_empty[slot]));
           }
         }
       }
-      ++j;
-      return true;
-    };
-    uint32_t done = 0;
-    bool ok = true;
-    auto store = [&](const Chunk& x) {
+    } else if (warp >= 12) {
+      // =========================== V: codes times scale -> 16 bits in the ring ===========================
+      // A warp has 32 rows, that is two steps of O^T += V^T P^T.
+      const int row0 = 32 * (warp - 12);
+      uint32_t n = 0;
+      bool ok = true;
+      while (ok) {
+        const PagedPiece it = take_item();
+        if (it.id < 0) break;
+  #pragma unroll 1
+        for (int j = 0; j < it.tiles; ++j, ++n) {
+          const uint32_t slot = n % kStages, at = 2 * n + 1, from = at % T::kCodeStages;
+          ok = rolled_wait_warp(smem_u32(&bar_code_full[from]), at / T::kCodeStages & 1, &abort_word, 22) &&
+               rolled_wait_warp(smem_u32(&bar_kv_empty[slot]), (n / kStages & 1) ^ 1, &abort_word, 23);
+          if (!ok) break;
+          const int rows = it.sk - (it.first + j) * 128 - row0;  // of the 32 that exist
+          const uint32_t my_scale = lane < rows ? scale_byte(from, row0 + lane) : 127u;
+          const uint32_t fits = __ballot_sync(0xffffffffu, my_scale >= 112 && my_scale <= 134);
+          const uint32_t from_smem = code_smem + from * T::kCodeBytes, to_smem = ring_smem + slot * T::kTileBytes;
+          const bool plain = fits == 0xffffffffu;
+#pragma unroll 1
+          for (int i = 0; i < T::kChunks; ++i) {
+            const int idx = lane + 32 * i, r = idx / T::kChunks, chunk = idx % T::kChunks, row = row0 + r;
+            const float4 f = lds128(from_smem + row * 128 + ((chunk ^ (row & 7)) << 4));
+            const uint32_t exists = r < rows ? 0xffffffffu : 0u;
+            const uint32_t codes[4] = {__float_as_uint(f.x) & exists, __float_as_uint(f.y) & exists,
+                                       __float_as_uint(f.z) & exists, __float_as_uint(f.w) & exists};
+            const uint32_t byte = __shfl_sync(0xffffffffu, my_scale, r);
+            uint32_t w[8];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t slot = done % kStages;
-        ok = ok && mbar_wait_warp(smem_u32(&bar_kv_empty[slot]), (done / kStages & 1) ^ 1, &abort_word, 16);
-        if (!ok) return;
+            for (int u = 0; u < 4; ++u) {
+              w[2 * u] = e4m3x2_to_half2(codes[u] & 0xffffu);
+              w[2 * u + 1] = e4m3x2_to_half2(codes[u] >> 16);
+            }
+            if (plain || (fits >> (r & 16) & 0xffffu) == 0xffffu) {
+              const uint32_t h = (byte == 112 ? 0x0200u : (byte - 112) << 10) * 0x10001u;  // 2^(byte - 127) in fp16, twice
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int idx = t + 256 * i, row = idx / T::kChunks, chunk = idx % T::kChunks;
-          const float s = scale_value(x.scale[n][i]);
-          const uint2 a = e4m3x4_to_16<kBf16>(x.codes[n][i].x, s), b = e4m3x4_to_16<kBf16>(x.codes[n][i].y, s);
-          const uint2 e = e4m3x4_to_16<kBf16>(x.codes[n][i].z, s), f = e4m3x4_to_16<kBf16>(x.codes[n][i].w, s);
-          const uint32_t base = ring_smem + slot * T::kTileBytes + (chunk >> 2) * T::kBoxBytes + row * 128;
-          const uint32_t q = (chunk & 3) * 2;
-          // (threads of the second box start with their second half: the two boxes have the same banks)
-          const bool swap = (chunk >> 2) != 0;
-          const uint32_t first = base + (((q + (swap ? 1 : 0)) ^ (row & 7)) << 4);
-          const uint32_t second = base + (((q + (swap ? 0 : 1)) ^ (row & 7)) << 4);
-          sts128(first, swap ? e.x : a.x, swap ? e.y : a.y, swap ? f.x : b.x, swap ? f.y : b.y);
-          sts128(second, swap ? a.x : e.x, swap ? a.y : e.y, swap ? b.x : f.x, swap ? b.y : f.y);
+              for (int u = 0; u < 8; ++u) w[u] = mul_half2(w[u], h);
+            } else {
+              const float s = scale_value(byte);
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const float2 v = __half22float2(*reinterpret_cast<__half2*>(&w[u]));
+                w[u] = pack16x2<kBf16>(v.x * s, v.y * s);
+              }
+            }
+            // (threads of the second box start with their second half: the two boxes have the same banks)
+            const bool swap = (chunk >> 2) != 0;
+            const uint32_t at16 = (((chunk & 3) * 2 + (swap ? 1 : 0)) ^ (row & 7)) << 4;
+            const uint32_t base = to_smem + (chunk >> 2) * T::kBoxBytes + row * 128;
+            sts128(base + at16, swap ? w[4] : w[0], swap ? w[5] : w[1], swap ? w[6] : w[2], swap ? w[7] : w[3]);
+            sts128(base + (at16 ^ 16), swap ? w[0] : w[4], swap ? w[1] : w[5], swap ? w[2] : w[6], swap ? w[3] : w[7]);
+          }
+          if (lane < 2) v_bf16[slot][2 * (warp - 12) + lane] = (fits >> (16 * lane) & 0xffffu) != 0xffffu;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(smem_u32(&bar_kv_full[slot]));
+            mbar_arrive(smem_u32(&bar_code_empty[from]));
+          }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_kv_full[slot]));
-        ++done;
-      }
-    };
-    bool have[kDepth];
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) have[d] = fetch(buf[d]);
-    while (ok && have[0]) {
-#pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        if (!ok || !have[d]) continue;
-        store(buf[d]);
-        have[d] = ok && fetch(buf[d]);
       }
     }
   }

@@ -6,7 +6,8 @@
 // block does of one item is a piece.  A piece that is its whole item writes O and LSE; others leave fp32 rows, which
 // paged_join_kernel joins.  So every SM has the same number of keys to read whatever the lengths are, a single long
 // entry is spread over all of them, and an item is cut about as often as there are blocks to an item, no more.
-// Every block works out the line's length and its own place on it from the lengths, a warp at a time.
+// Every block works out the line's length and its own place on it from the lengths, a warp at a time.  (The line
+// has less than 2^31 units: checked on the host.)
 #pragma once
 #include "cache_kernels.cuh"
 
@@ -16,14 +17,17 @@ struct PagedParams {
   PagedCache cache;
   const int32_t *seqused_k, *seqused_q;
   int batch, heads_k, group, seqlen_q, causal;
+  unsigned group_mul;     // r / group = (r * group_mul) >> 16 for r < 256
   int blocks_per_entry;   // blocks of new tokens
   int tokens_per_block;
   int box_rows;           // rows of a K or V box: what divides both a page and a tile
   int min_share;          // units a block has at least
   float scale_log2;       // |scale| * log2(e)
   int negate;             // scale < 0: the tensor cores form -Q K^T
+  const uint16_t* q;
+  long long q_batch, q_row, q_head;  // element strides
   uint16_t* o;
-  long long o_batch, o_row, o_head;  // element strides
+  long long o_batch, o_row, o_head;
   float* lse;
   // workspace: rows of pieces (slot, row, DR), their log-sum-exp (slot, row), blocks of every item
   float *o_part, *lse_part;
@@ -56,41 +60,50 @@ __device__ __forceinline__ int paged_tiles(const PagedParams& p, int token0, int
   return (paged_last_key(p, min(token0 + p.tokens_per_block, sq) - 1, sq, sk) + 128) / 128;
 }
 
+__device__ __forceinline__ int row_token(const PagedParams& p, int r) { return (int)((unsigned)r * p.group_mul >> 16); }
+
 // One block's share, walked in order by a converged warp (every lane has the same state).
 struct PagedWork {
-  long long pos, end;      // units still to do
-  long long pair_start;    // first unit of the current (entry, block of tokens), all heads of which follow
-  int pair, tiles;
+  int pos, end;     // units still to do
+  int pair_start;   // first unit of the current (entry, block of tokens), all heads of which follow
+  int pair, z, token0, tiles;
   int sq, sk;
-  long long share;
+  int share;
 
-  __device__ __forceinline__ int pair_tiles(const PagedParams& p, int f, int& q, int& k) const {
-    paged_lengths(p, f / p.blocks_per_entry, q, k);
-    return paged_tiles(p, f % p.blocks_per_entry * p.tokens_per_block, q, k);
+  // (calls, not inlined: they run once a piece, and the instruction cache is what the roles of a block share)
+  __device__ __forceinline__ void enter_pair(const PagedParams& p) {
+    z = pair / p.blocks_per_entry;
+    token0 = (pair - z * p.blocks_per_entry) * p.tokens_per_block;
+    paged_lengths(p, z, sq, sk);
+    tiles = paged_tiles(p, token0, sq, sk);
   }
 
-  __device__ __forceinline__ void start(const PagedParams& p, int block, int blocks) {
+  __device__ __noinline__ void start(const PagedParams& p, int block, int blocks) {
     const int lane = threadIdx.x & 31;
     const int pairs = p.batch * p.blocks_per_entry;
-    auto units = [&](int f) -> long long {
-      int q, k;
-      return f < pairs ? (long long)p.heads_k * (pair_tiles(p, f, q, k) + kItemCost) : 0;
+    auto units = [&](int f) {
+      if (f >= pairs) return 0;
+      pair = f;
+      enter_pair(p);
+      return p.heads_k * (tiles + kItemCost);
     };
-    long long total = 0;
+    int total = 0;
+#pragma unroll 1
     for (int f = lane; f < pairs; f += 32) total += units(f);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-    share = max((long long)p.min_share, (total + blocks - 1) / blocks);
+    total = __reduce_add_sync(0xffffffffu, total);
+    share = max(p.min_share, (int)(((unsigned)total + blocks - 1) / blocks));
+    pos = end = 0;
+    if ((long long)block * share >= total) return;
     pos = block * share;
-    end = min(pos + share, total);
-    if (pos >= end) return;
-    long long before = 0;  // units of the pairs before this group of 32
+    end = share < total - pos ? pos + share : total;
+    int before = 0;  // units of the pairs before this group of 32
+#pragma unroll 1
     for (int f0 = 0;; f0 += 32) {
-      const long long mine = units(f0 + lane);
-      long long sum = mine;
+      const int mine = units(f0 + lane);
+      int sum = mine;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, sum, off);
+        const int up = __shfl_up_sync(0xffffffffu, sum, off);
         if (lane >= off) sum += up;
       }
       const uint32_t beyond = __ballot_sync(0xffffffffu, before + sum > pos);
@@ -102,37 +115,38 @@ struct PagedWork {
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    tiles = pair_tiles(p, pair, sq, sk);
+    enter_pair(p);
   }
 
-  __device__ __forceinline__ PagedPiece next(const PagedParams& p, int block) {
+  __device__ __noinline__ PagedPiece next(const PagedParams& p, int block) {
     PagedPiece it;
     it.id = -1;
     it.tiles = 0;
+#pragma unroll 1
     while (pos < end) {
       const int w = tiles + kItemCost;
-      if (pos - pair_start >= (long long)p.heads_k * w) {
-        pair_start += (long long)p.heads_k * w;
+      const int h = (pos - pair_start) / w;
+      if (h >= p.heads_k) {
+        pair_start += p.heads_k * w;
         ++pair;
-        tiles = pair_tiles(p, pair, sq, sk);
+        enter_pair(p);
         continue;
       }
-      const int h = (int)((pos - pair_start) / w);
-      const long long u0 = pair_start + (long long)h * w;
-      const int first = (int)(pos - u0), last = (int)min((long long)tiles, end - u0);
+      const int u0 = pair_start + h * w;
+      const int first = pos - u0, last = min(tiles, end - u0);
       pos = u0 + w;
       if (first >= tiles && !(tiles == 0 && first == 0)) continue;  // only the item's end: nothing to do for it
       it.id = pair * p.heads_k + h;
-      it.z = pair / p.blocks_per_entry;
+      it.z = z;
       it.h = h;
-      it.token0 = pair % p.blocks_per_entry * p.tokens_per_block;
+      it.token0 = token0;
       it.first = first;
       it.tiles = last - first;
       it.slot = first == 0 && last == tiles ? -1 : 2 * block + (first > 0 ? 0 : 1);
       it.sq = sq;
       it.sk = sk;
       if (first == 0 && (threadIdx.x & 31) == 0)
-        p.item_blocks[it.id] = make_int2((int)(u0 / share), tiles > 0 ? (int)((u0 + tiles - 1) / share) : (int)(u0 / share));
+        p.item_blocks[it.id] = make_int2(u0 / share, tiles > 0 ? (u0 + tiles - 1) / share : u0 / share);
       break;
     }
     return it;
@@ -154,7 +168,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, in
   if (blocks.x < 0 || blocks.x >= blocks.y || blocks.y >= blocks_of_grid) return;
   const int h = item % p.heads_k, pair = item / p.heads_k;
   const int z = pair / p.blocks_per_entry;
-  const int token = pair % p.blocks_per_entry * p.tokens_per_block + row / p.group, hq = h * p.group + row % p.group;
+  const int token_in_block = row_token(p, row);
+  const int token = pair % p.blocks_per_entry * p.tokens_per_block + token_in_block;
+  const int hq = h * p.group + row - token_in_block * p.group;
   if (token >= p.seqlen_q) return;
   auto slot = [&](int b) { return b == blocks.x ? 2 * b + 1 : 2 * b; };
   // a part that is NaN makes the row NaN

@@ -101,6 +101,20 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
+// The same with a loop that the compiler does not unroll (four polls in a row are 20 instructions more per wait), for
+// kernels whose roles have to share the instruction cache
+__device__ __forceinline__ bool rolled_wait(uint32_t bar, uint32_t parity, volatile int* abort_word, int who) {
+#pragma unroll 1
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+    if (*abort_word != 0) return false;
+    if (i == kWaitPollLimit) {
+      *abort_word = kErrWaitTimeout | (who & 0xff);
+      return false;
+    }
+  }
+  return true;
+}
+
 // Bounded wait for a field of a word in global memory, (word >> shift) & mask, to reach `want` (modulo the field);
 // another CTA of the same grid adds to it (global_flag_release), for an item that was handed out before this one's.
 // Gives up at once when this CTA, or the grid (status word), is already aborting.
@@ -149,6 +163,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void* src, ui
                :
                : "r"(dst_smem), "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+// asynchronous copy of an aligned word to shared memory, and an arrival on a barrier when all of the thread's are there
+__device__ __forceinline__ void copy_async4(uint32_t dst_smem, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst_smem), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tma_store_4d(const void* tmap, uint32_t src_smem, int c0, int c1,
                                              int c2, int c3) {
@@ -378,6 +399,11 @@ __device__ __forceinline__ void umma_commit_elect(uint32_t bar) {
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity,
                                                volatile int* abort_word, int who) {
   const bool ok = mbar_wait(bar, parity, abort_word, who);
+  return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ bool rolled_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_word, int who) {
+  const bool ok = rolled_wait(bar, parity, abort_word, who);
   return __all_sync(0xffffffffu, ok);
 }
 
