@@ -37,9 +37,12 @@ __device__ __forceinline__ int cache_page_row(const PagedCache& c, int t) {
 // tokens an entry can hold at most (fits: checked on the host)
 __device__ __forceinline__ int cache_capacity(const PagedCache& c) { return c.max_pages * c.page_size; }
 
-// the page of token `t` of entry z, -1 where the table names none
+// what the table has for token `t` of entry z; its page, -1 where the table names none
+__device__ __forceinline__ int cache_entry(const PagedCache& c, int z, int t) {
+  return __ldg(c.table + z * c.table_stride + cache_page_index(c, t));
+}
 __device__ __forceinline__ int cache_page(const PagedCache& c, int z, int t) {
-  const int page = __ldg(c.table + z * c.table_stride + cache_page_index(c, t));
+  const int page = cache_entry(c, z, t);
   return (unsigned)page < (unsigned)c.num_pages ? page : -1;
 }
 

@@ -119,13 +119,17 @@ int make_pool_map(CUtensorMap* map, const void* base, const FmhaPagedCache& c, c
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)c.page_size, (cuuint64_t)heads, (cuuint64_t)c.num_pages};
   const cuuint64_t strides[3] = {(cuuint64_t)row * unit, (cuuint64_t)head * unit, (cuuint64_t)page * unit};
   const cuuint32_t box[4] = {codes ? 128u : 64u, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  // What a miss brings into the L2 is no more than a row has: the row behind it is another head's, which another block reads
+  // at another time.
+  const CUtensorMapL2promotion promotion = D * unit >= 256   ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                           : D * unit >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                                             : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
   const CUresult r = encode(map,
                             codes  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                             : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                             4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                            CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FMHA_OK : FMHA_ERR_TENSOR_MAP;
 }
 

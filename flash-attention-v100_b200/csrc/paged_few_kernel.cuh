@@ -11,8 +11,8 @@
 // across threads, only a vote.
 //
 //   warps 0-3   softmax: thread = key; P^T to shared memory; O^T (thread = element of the head) at the end
-//   warp 4      MMA issuer
-//   warp 5      producer of Q
+//   warps 4, 7  MMA issuers, of S^T and of O^T
+//   warp 5      producer of Q; 8-bit caches: of the scales
 //   warp 6      source of pieces; TMA producer of K and V, a box per page (or per part of one)
 // 8-bit caches, whose codes and scales arrive in a ring of their own:
 //   warps 8-11  K: codes -> fp16, into tensor memory (a thread has a key there, as in the softmax)
@@ -54,7 +54,7 @@ struct FewTraits {
   static constexpr int kCodeBytes = 128 * 128;
   static constexpr int kQBufs = D == 128 && (kRows == 64 || (kE4m3 && kRows == 32)) ? 1 : 2;
   static constexpr int kItemStages = 8;
-  static constexpr int kThreads = kE4m3 ? 512 : 224;
+  static constexpr int kThreads = kE4m3 ? 512 : 256;
   static constexpr int kSmemBytes =
       1024 + kStages * kTileBytes + kCodeStages * kCodeBytes + kQBufs * kQBytes + 2 * kPBytes;
   static constexpr int kTmemCols = !kE4m3 ? 4 * kRows : kRows == 64 ? 512 : 256;
@@ -162,14 +162,14 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   if (threadIdx.x == 0) {
     for (int s = 0; s < T::kItemStages; ++s) {
       mbar_init(smem_u32(&bar_item_full[s]), 1);
-      mbar_init(smem_u32(&bar_item_empty[s]), kE4m3 ? 14 : 6);  // MMA, Q, four softmax (eight converting) warps
+      mbar_init(smem_u32(&bar_item_empty[s]), kE4m3 ? 15 : 7);  // two MMA, Q, four softmax (eight converting) warps
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&bar_kv_full[s]), kE4m3 ? 4 : 1);
       mbar_init(smem_u32(&bar_kv_empty[s]), 1);
     }
     for (int s = 0; s < T::kCodeStages; ++s) {
-      mbar_init(smem_u32(&bar_code_full[s]), 33);  // TMA's thread, a warp's copies of scales
+      mbar_init(smem_u32(&bar_code_full[s]), 34);  // TMA's thread, a warp's copies of scales, its word on which byte
       mbar_init(smem_u32(&bar_code_empty[s]), 4);
     }
     for (int b = 0; b < 2; ++b) {
@@ -225,92 +225,105 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     return code_scale[stage][row] >> ((code_select[stage][row >> 2] >> (row % 4 * 2) & 3) * 8) & 0xffu;
   };
 
+  // Pages of a piece's tiles, in parts of box_rows rows, 32 parts at a time, a lane each, and the next 32 while these are used:
+  // a lookup takes microseconds when all of HBM's rate is used.
+  const int subs = 128 / p.box_rows;
+  struct Pages {
+    int now, next;
+  };
+  // the table's entry for part 32 * batch + lane (not looked at before it is used)
+  auto lookup = [&](const PagedPiece& it, int batch) {
+    const int part = 32 * batch + lane, key = it.first * 128 + part * p.box_rows;
+    int entry = -1;
+    if (part < it.tiles * subs && key < it.sk) entry = cache_entry(p.cache, it.z, key);
+    return entry;
+  };
+  // the page of a part of tile j, j in ascending order (num_pages, outside the pool, where there is none)
+  auto page_of = [&](const PagedPiece& it, Pages& w, int j, int sub) {
+    if (j > 0 && j * subs % 32 == 0) {
+      w.now = w.next;
+      w.next = lookup(it, j * subs / 32 + 1);
+    }
+    const int page = __shfl_sync(0xffffffffu, w.now, (j * subs + sub) & 31);
+    return (unsigned)page < (unsigned)p.cache.num_pages ? page : p.cache.num_pages;
+  };
+
   if (warp == 6) {
     // =========================== source of pieces, K and V producer ===========================
-    // a lane per box: 128 / box_rows parts of a tile, kBoxes column blocks of each (codes: one)
+    // A lane per box: 128 / box_rows parts of a tile, kBoxes column blocks of each (codes: one); lanes 0-15 K's, 16-31 V's.
+    // One pass of the loop for both, because the pass, not what it asks for, is what takes the time (500 clk).  The next
+    // piece is worked out while the last tiles of this one are asked for.
     constexpr int kCols = kE4m3 ? 1 : T::kBoxes;
     constexpr uint32_t kRing = kE4m3 ? T::kCodeStages : kStages;
     constexpr uint32_t kBytes = kE4m3 ? T::kCodeBytes : T::kTileBytes;
-    const int sub = lane / kCols, box = lane % kCols;
-    const bool mine = sub < 128 / p.box_rows;
+    const bool is_v = lane >= 16;
+    const int sub = (lane & 15) / kCols, box = lane % kCols;
+    const bool mine = sub < subs;
     const uint32_t dst = (kE4m3 ? code_smem : ring_smem) + box * T::kBoxBytes + sub * p.box_rows * 128;
+    const CUtensorMap* const tm = is_v ? &tm_v : &tm_k;
+    uint64_t* const fulls = kE4m3 ? bar_code_full : bar_kv_full;
+    uint64_t* const empties = kE4m3 ? bar_code_empty : bar_kv_empty;
     PagedWork work;
     work.start(p, blockIdx.x, gridDim.x);
     bool ok = true;
     uint32_t slot = 0, phase = 1, published = 0;
-    while (ok) {
-      const PagedPiece it = work.next(p, blockIdx.x);
+    auto next_item = [&]() -> PagedPiece {
+      PagedPiece it = work.next(p, blockIdx.x);
       const uint32_t s = published % T::kItemStages, round = published / T::kItemStages;
-      if (round > 0 && !rolled_wait_warp(smem_u32(&bar_item_empty[s]), (round - 1) & 1, &abort_word, 2)) break;
-      if (lane == 0) {
+      if (round > 0) ok = rolled_wait_warp(smem_u32(&bar_item_empty[s]), (round - 1) & 1, &abort_word, 2);
+      if (ok && lane == 0) {
         items[s] = it;
         mbar_arrive(smem_u32(&bar_item_full[s]));
       }
       __syncwarp();
       ++published;
-      if (it.id < 0) break;
-      auto place = [&](int tile, int& row) {  // page of this lane's part (num_pages, outside the pool: zeros)
-        const int key = (it.first + tile) * 128 + sub * p.box_rows;
-        row = cache_page_row(p.cache, key);
-        if (!mine || key >= it.sk) return p.cache.num_pages;
-        const int page = cache_page(p.cache, it.z, key);
-        return page < 0 ? p.cache.num_pages : page;
-      };
-      int row_next = 0, page_next = 0;
+      return it;
+    };
+    PagedPiece it = next_item();
+    Pages pages;
+    pages.now = lookup(it, 0);
+    while (ok && it.id >= 0) {
+      PagedPiece after = it;
+      int pages_after = 0;
+      pages.next = lookup(it, 1);
 #pragma unroll 1
-      for (int j = -1; ok && j < it.tiles; ++j) {
-        const int row = row_next, page = page_next;
-        if (j + 1 < it.tiles) page_next = place(j + 1, row_next);
-        if (j < 0) continue;
-#pragma unroll 1
-        for (int n = 0; n < 2; ++n) {
-          uint64_t* const full = kE4m3 ? &bar_code_full[slot] : &bar_kv_full[slot];
-          uint64_t* const empty = kE4m3 ? &bar_code_empty[slot] : &bar_kv_empty[slot];
-          if (!(ok = rolled_wait_warp(smem_u32(empty), phase, &abort_word, 3))) break;
-          if constexpr (kE4m3) {
-            // scales: four rows a lane, in one page; the copy is of words, each the one that a row's byte is in (a
-            // word that holds a byte of an allocation is in it)
-            const int from = lane * 4 / p.box_rows, page4 = __shfl_sync(0xffffffffu, page, from);
-            const long long row4 = __shfl_sync(0xffffffffu, row, from) + lane * 4 % p.box_rows;
-            const PagePool& pool = n ? p.cache.v : p.cache.k;
-            const uint8_t* src = pool.scales + page4 * pool.scale_page + row4 * pool.scale_row + it.h * pool.scale_head;
-            const uint32_t to = smem_u32(&code_scale[slot][lane * 4]);
-            uint32_t select = 0;
-            if (page4 < p.cache.num_pages) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i, src += pool.scale_row) {
-                const size_t at = reinterpret_cast<size_t>(src);
-                copy_async4(to + 4 * i, reinterpret_cast<const void*>(at & ~size_t(3)));
-                select |= (uint32_t)(at & 3) << (2 * i);
-              }
-            } else {
-              sts128(to, 127, 127, 127, 127);
-            }
-            code_select[slot][lane] = (uint8_t)select;
-            copy_async_arrive(smem_u32(full));
-            __syncwarp();
-          }
-          if (lane == 0) mbar_arrive_expect_tx(smem_u32(full), kBytes);
-          __syncwarp();
-          if (mine) tma_load_4d(dst + slot * kBytes, n ? &tm_v : &tm_k, smem_u32(full), box * 64, row, it.h, page);
-          __syncwarp();
-          if (++slot == kRing) {
-            slot = 0;
-            phase ^= 1;
-          }
+      for (int j = 0; ok && j < max(it.tiles, 1); ++j) {
+        if (j + 2 >= it.tiles && after.id == it.id) {
+          after = next_item();
+          pages_after = lookup(after, 0);
         }
+        if (j >= it.tiles) break;  // (no tiles at all)
+        const int page = page_of(it, pages, j, sub);
+        const int row = cache_page_row(p.cache, it.first * 128 + (j * subs + sub) * p.box_rows);
+        // K's slot and V's, the one behind it
+        const uint32_t slot_v = slot + 1 == kRing ? 0 : slot + 1, phase_v = slot + 1 == kRing ? phase ^ 1 : phase;
+        ok = ok && rolled_wait_warp(smem_u32(&empties[slot]), phase, &abort_word, 3) &&
+             rolled_wait_warp(smem_u32(&empties[slot_v]), phase_v, &abort_word, 4);
+        if (!ok) break;
+        const uint32_t to = is_v ? slot_v : slot, full = smem_u32(&fulls[to]);
+        if ((lane & 15) == 0) mbar_arrive_expect_tx(full, kBytes);
+        __syncwarp();
+        if (mine) tma_load_4d(dst + to * kBytes, tm, full, box * 64, row, it.h, page);
+        __syncwarp();
+        phase = slot + 2 >= kRing ? phase ^ 1 : phase;
+        slot = slot + 2 >= kRing ? slot + 2 - kRing : slot + 2;
       }
+      it = after;
+      pages.now = pages_after;
     }
   } else if (warp == 5) {
-    // =========================== Q producer ===========================
+    // =========================== Q producer; scales of codes ===========================
     const uint32_t bytes = T::kBoxes * p.seqlen_q * p.group * 128;
     uint32_t used = 0;
+    [[maybe_unused]] uint32_t slot = 0, phase = 1;
     for (;;) {
       const PagedPiece it = take_item();
       if (it.id < 0) break;
       if (it.tiles == 0) continue;
+      [[maybe_unused]] Pages pages = {};
+      if constexpr (kE4m3) pages = {lookup(it, 0), lookup(it, 1)};
       const uint32_t b = used % T::kQBufs, round = used / T::kQBufs;
-      if (round > 0 && !rolled_wait_warp(smem_u32(&bar_q_free[b]), (round - 1) & 1, &abort_word, 4)) break;
+      if (round > 0 && !rolled_wait_warp(smem_u32(&bar_q_free[b]), (round - 1) & 1, &abort_word, 24)) break;
       if constexpr (kE4m3 && kBf16) {
         // Q in fp16, like K: divided by the power of two that brings its largest value to [2^14, 2^15).  What is less
         // than 2^-28 of that value loses bits, nothing is off by more than 2^-39 of it.
@@ -354,58 +367,62 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       }
       __syncwarp();
       ++used;
+      if constexpr (kE4m3) {
+        // Four rows a lane, in one page; the copy is of words, each the one that a row's byte is in (a word that holds a
+        // byte of an allocation is in it).
+        const int sub = lane * 4 / p.box_rows, in_part = lane * 4 % p.box_rows;
+        bool ok = true;
+#pragma unroll 1
+        for (int j = 0; j < it.tiles; ++j) {
+          const int page = page_of(it, pages, j, sub);
+          const long long row = cache_page_row(p.cache, it.first * 128 + (j * subs + sub) * p.box_rows) + in_part;
+#pragma unroll 1
+          for (int n = 0; n < 2; ++n) {
+            const PagePool& pool = n ? p.cache.v : p.cache.k;
+            const uint8_t* src = pool.scales + page * pool.scale_page + row * pool.scale_row + it.h * pool.scale_head;
+            ok = ok && rolled_wait_warp(smem_u32(&bar_code_empty[slot]), phase, &abort_word, 19);
+            if (!ok) break;
+            const uint32_t to = smem_u32(&code_scale[slot][lane * 4]);
+            uint32_t select = 0;
+            if (page < p.cache.num_pages) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i, src += pool.scale_row) {
+                const size_t at = reinterpret_cast<size_t>(src);
+                copy_async4(to + 4 * i, reinterpret_cast<const void*>(at & ~size_t(3)));
+                select |= (uint32_t)(at & 3) << (2 * i);
+              }
+            } else {
+              sts128(to, 127, 127, 127, 127);
+            }
+            code_select[slot][lane] = (uint8_t)select;
+            copy_async_arrive(smem_u32(&bar_code_full[slot]));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bar_code_full[slot]));
+            if (++slot == (uint32_t)T::kCodeStages) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
+        }
+        if (!ok) break;
+      }
     }
   } else if (warp == 4) {
-    // =========================== MMA issuer ===================
-    // S^T of a tile is issued before O^T of the one before it, so that the tensor pipe has work while the softmax
-    // warps have the tile.  K of tile n is slot 2n of the ring, V slot 2n + 1.
-    uint32_t n = 0, piece = 0;
+    // =========================== MMA issuer of S^T = K Q^T ===================
+    // Each product has a warp of its own: issuing, the commits most of all, takes longer than the products themselves.
+    uint32_t n = 0, piece = 0, slot = 0, phase = 0;
     bool ok = true;
-    bool pending = false, pending_first = false, pending_last = false;
-    uint32_t pending_piece = 0;
-    auto issue_pv = [&]() {
-      const uint32_t m = n - 1, b = m & 1, at = v_at(m), slot = at % kStages;
-      ok = rolled_wait_warp(smem_u32(&bar_p_full[b]), (m >> 1) & 1, &abort_word, 5) &&
-           rolled_wait_warp(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 6);
-      const uint32_t ob = pending_piece & 1;
-      if (ok && pending_first && pending_piece >= 2)
-        ok = rolled_wait_warp(smem_u32(&bar_o_free[ob]), ((pending_piece >> 1) - 1) & 1, &abort_word, 7);
-      if (!ok) return;
-      tc_fence_after();
-      const uint32_t a_lo = umma_desc_lo(ring_smem + slot * T::kTileBytes, T::kLboV);
-      const uint32_t b_lo = umma_desc_lo(p_smem + b * T::kPBytes, kLboKMajor);
-      uint2 in_bf16 = make_uint2(0, 0);  // a byte for each 16 keys
-      if constexpr (kE4m3 && kBf16) {
-        in_bf16 = *reinterpret_cast<const uint2*>(v_bf16[slot]);
-        in_bf16.x = __shfl_sync(0xffffffffu, in_bf16.x, 0);
-        in_bf16.y = __shfl_sync(0xffffffffu, in_bf16.y, 0);
-      }
-      if (elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const bool bf = ((ks < 4 ? in_bf16.x : in_bf16.y) >> (ks % 4 * 8) & 1) != 0;
-          umma_ss(tmem_base + (2 + ob) * kRows, a_lo + ((ks * 2048) >> 4),
-                  b_lo + (((ks >> 2) * kRows * 128 + (ks & 3) * 32) >> 4), bf ? T::kIdescPVBf16 : T::kIdescPV,
-                  (!pending_first || ks > 0) ? 1u : 0u);
-        }
-        umma_commit(smem_u32(&bar_kv_empty[slot]));
-        umma_commit(smem_u32(&bar_p_free[b]));
-        if (pending_last) umma_commit(smem_u32(&bar_o_full[ob]));
-      }
-      __syncwarp();
-      pending = false;
-    };
     while (ok) {
       const PagedPiece it = take_item();
       if (it.id < 0) break;
 #pragma unroll 1
-      for (int j = 0; j < it.tiles; ++j) {
-        const uint32_t b = n & 1, at = 2 * n, slot = at % kStages, qb = piece % T::kQBufs;
+      for (int j = 0; j < it.tiles; ++j, ++n) {
+        const uint32_t b = n & 1, qb = piece % T::kQBufs;
         if (j == 0) ok = rolled_wait_warp(smem_u32(&bar_q_full[qb]), piece / T::kQBufs & 1, &abort_word, 8);
         if (kE4m3)
           ok = ok && rolled_wait_warp(smem_u32(&bar_kt_full[b]), (n >> 1) & 1, &abort_word, 18);
         else
-          ok = ok && rolled_wait_warp(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 9);
+          ok = ok && rolled_wait_warp(smem_u32(&bar_kv_full[slot]), phase, &abort_word, 9);
         if (ok && n >= 2) ok = rolled_wait_warp(smem_u32(&bar_s_free[b]), ((n >> 1) - 1) & 1, &abort_word, 10);
         if (!ok) break;
         tc_fence_after();
@@ -421,22 +438,62 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
               umma_ss(tmem_base + b * kRows, a_lo + (((ks >> 2) * T::kBoxBytes + (ks & 3) * 32) >> 4), q_lo, T::kIdescQK,
                       ks > 0 ? 1u : 0u);
           }
-          umma_commit(smem_u32(kE4m3 ? &bar_kt_free[b] : &bar_kv_empty[slot]));
           umma_commit(smem_u32(&bar_s_full[b]));
+          umma_commit(smem_u32(kE4m3 ? &bar_kt_free[b] : &bar_kv_empty[slot]));
           if (j == it.tiles - 1) umma_commit(smem_u32(&bar_q_free[qb]));
         }
         __syncwarp();
-        if (pending) issue_pv();
-        if (!ok) break;
-        ++n;
-        pending = true;
-        pending_first = j == 0;
-        pending_last = j == it.tiles - 1;
-        pending_piece = piece;
+        if ((slot += 2) >= (uint32_t)kStages) {
+          slot -= kStages;
+          phase ^= 1;
+        }
       }
       if (it.tiles > 0) ++piece;
     }
-    if (ok && pending) issue_pv();
+  } else if (warp == 7) {
+    // =========================== MMA issuer of O^T += V^T P^T ===================
+    uint32_t n = 0, piece = 0, slot = kE4m3 ? 0 : 1, phase = 0;
+    bool ok = true;
+    while (ok) {
+      const PagedPiece it = take_item();
+      if (it.id < 0) break;
+      const uint32_t ob = piece & 1;
+#pragma unroll 1
+      for (int j = 0; j < it.tiles; ++j, ++n) {
+        const uint32_t b = n & 1;
+        if (j == 0 && piece >= 2) ok = rolled_wait_warp(smem_u32(&bar_o_free[ob]), ((piece >> 1) - 1) & 1, &abort_word, 7);
+        ok = ok && rolled_wait_warp(smem_u32(&bar_kv_full[slot]), phase, &abort_word, 6) &&
+             rolled_wait_warp(smem_u32(&bar_p_full[b]), (n >> 1) & 1, &abort_word, 5);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t a_lo = umma_desc_lo(ring_smem + slot * T::kTileBytes, T::kLboV);
+        const uint32_t b_lo = umma_desc_lo(p_smem + b * T::kPBytes, kLboKMajor);
+        uint2 in_bf16 = make_uint2(0, 0);  // a byte for each 16 keys
+        if constexpr (kE4m3 && kBf16) {
+          in_bf16 = *reinterpret_cast<const uint2*>(v_bf16[slot]);
+          in_bf16.x = __shfl_sync(0xffffffffu, in_bf16.x, 0);
+          in_bf16.y = __shfl_sync(0xffffffffu, in_bf16.y, 0);
+        }
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const bool bf = ((ks < 4 ? in_bf16.x : in_bf16.y) >> (ks % 4 * 8) & 1) != 0;
+            umma_ss(tmem_base + (2 + ob) * kRows, a_lo + ((ks * 2048) >> 4),
+                    b_lo + (((ks >> 2) * kRows * 128 + (ks & 3) * 32) >> 4), bf ? T::kIdescPVBf16 : T::kIdescPV,
+                    (j > 0 || ks > 0) ? 1u : 0u);
+          }
+          umma_commit(smem_u32(&bar_kv_empty[slot]));
+          umma_commit(smem_u32(&bar_p_free[b]));
+          if (j == it.tiles - 1) umma_commit(smem_u32(&bar_o_full[ob]));
+        }
+        __syncwarp();
+        if ((slot += kE4m3 ? 1 : 2) >= (uint32_t)kStages) {
+          slot -= kStages;
+          phase ^= 1;
+        }
+      }
+      if (it.tiles > 0) ++piece;
+    }
   } else if (warp < 4) {
     // =========================== softmax, O ===========================
     const int tid = threadIdx.x;  // key of the tile, element of the head
@@ -671,7 +728,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           tc_fence_after();
           const uint32_t src = code_smem + slot * T::kCodeBytes + tid * 128;
           k_scale[n & 3][tid] = (uint8_t)scale_byte(slot, tid);
-  #pragma unroll 1
+  #pragma unroll 2
           for (int i = 0; i < T::kChunks; i += 2) {  // 32 elements, 16 columns of tensor memory
             uint32_t w[16];
 #pragma unroll
@@ -715,7 +772,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           const uint32_t fits = __ballot_sync(0xffffffffu, my_scale >= 112 && my_scale <= 134);
           const uint32_t from_smem = code_smem + from * T::kCodeBytes, to_smem = ring_smem + slot * T::kTileBytes;
           const bool plain = fits == 0xffffffffu;
-#pragma unroll 1
+          // (one warp per scheduler does this: what hides its latencies is the next chunks)
+#pragma unroll(T::kChunks == 8 ? 4 : T::kChunks / 2)
           for (int i = 0; i < T::kChunks; ++i) {
             const int idx = lane + 32 * i, r = idx / T::kChunks, chunk = idx % T::kChunks, row = row0 + r;
             const float4 f = lds128(from_smem + row * 128 + ((chunk ^ (row & 7)) << 4));
