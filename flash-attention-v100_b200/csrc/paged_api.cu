@@ -13,7 +13,7 @@
 #include "cache_kernels.cuh"
 #include "host_common.cuh"
 #include "paged_few_kernel.cuh"
-#include "paged_simple_kernel.cuh"
+#include "paged_many_kernel.cuh"
 
 namespace {
 
@@ -155,6 +155,8 @@ int make_rows_map(CUtensorMap* map, const void* base, int Z, int N, int H, int D
 struct PagedPlan {
   int kernel_rows;       // rows of an item that the kernel has room for
   int tokens_per_block;  // new tokens of an item
+  int rows_per_tile;     // rows in use of each of
+  int tiles;             // its row tiles
   int blocks_per_entry;
   int min_share;
   int blocks;            // of the grid
@@ -162,16 +164,25 @@ struct PagedPlan {
   size_t bytes() const { return part_bytes + lse_bytes + item_bytes; }
 };
 
-// Rows of up to 16, 32 or 64 run the kernel of few rows.
+// Rows (new tokens times query heads of a cache head) of up to 16, 32 or 64 run the kernel of few rows, more the one of many.
 PagedPlan plan_paged(const FmhaPagedFwdParams* p, int sms) {
   PagedPlan plan = {};
   const int group = p->heads_q / p->heads_k;
   const long long rows = (long long)p->seqlen_q * group;
-  if (rows > 64) return plan;
-  plan.kernel_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  plan.tokens_per_block = p->seqlen_q;
-  plan.blocks_per_entry = 1;
-  plan.min_share = 2;
+  if (rows <= 64) {
+    plan.kernel_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    plan.tokens_per_block = p->seqlen_q;
+    plan.rows_per_tile = (int)rows;
+    plan.tiles = 1;
+    plan.min_share = 2;
+  } else {
+    plan.kernel_rows = 256;
+    plan.tokens_per_block = 128 / group * 2;
+    plan.rows_per_tile = 128 / group * group;
+    plan.tiles = 2;
+    plan.min_share = 4;
+  }
+  plan.blocks_per_entry = (p->seqlen_q + plan.tokens_per_block - 1) / plan.tokens_per_block;
   plan.blocks = sms;
   const size_t items = (size_t)p->batch * plan.blocks_per_entry * p->heads_k;
   plan.part_bytes = (size_t)2 * plan.blocks * plan.kernel_rows * p->head_dim * sizeof(float);
@@ -193,7 +204,10 @@ fmha::PagedParams kernel_params(const FmhaPagedFwdParams* p, const PagedPlan& pl
   a.causal = p->causal ? 1 : 0;
   a.blocks_per_entry = plan.blocks_per_entry;
   a.tokens_per_block = plan.tokens_per_block;
+  a.rows_per_tile = plan.rows_per_tile;
   a.box_rows = std::gcd(p->cache.page_size, 128);
+  a.part_shift = 0;
+  while (a.box_rows << a.part_shift < 128) ++a.part_shift;
   a.min_share = plan.min_share;
   a.scale_log2 = std::fabs(p->scale) * 1.4426950408889634f;
   a.negate = p->scale < 0.f;
@@ -217,9 +231,9 @@ fmha::PagedParams kernel_params(const FmhaPagedFwdParams* p, const PagedPlan& pl
 // joins what was cut, launched as soon as no block of the kernel before is left to start or run (it waits for
 // their writes itself)
 template <bool kBf16, int DR, int kRows>
-int launch_join(const fmha::PagedParams& a, const PagedPlan& plan, int rows_per_item, cudaStream_t stream) {
+int launch_join(const fmha::PagedParams& a, const PagedPlan& plan, cudaStream_t stream) {
   using E = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
-  const int items = a.batch * a.blocks_per_entry * a.heads_k;
+  const int items = a.batch * a.blocks_per_entry * a.heads_k, rows_per_item = plan.tiles * plan.rows_per_tile;
   const long long rows = (long long)items * rows_per_item;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -252,7 +266,25 @@ int launch_few(const FmhaPagedFwdParams* p, const PagedPlan& plan, void* workspa
   if (!launch_with_smem<fmha::paged_few_kernel<D, DR, kBf16, kE4m3, kRows>>(dev, plan.blocks, T::kThreads, T::kSmemBytes,
                                                                             stream, tq, tk, tv, a))
     return FMHA_ERR_LAUNCH;
-  return launch_join<kBf16, DR, kRows>(a, plan, p->seqlen_q * a.group, stream);
+  return launch_join<kBf16, DR, kRows>(a, plan, stream);
+}
+
+template <int D, int DR, bool kBf16, bool kE4m3>
+int launch_many(const FmhaPagedFwdParams* p, const PagedPlan& plan, void* workspace, int dev, cudaStream_t stream) {
+  using T = fmha::ManyTraits<D, DR, kBf16, kE4m3>;
+  const fmha::PagedParams a = kernel_params(p, plan, workspace);
+  const int tokens = plan.tokens_per_block / 2;
+  CUtensorMap tq, tk, tv, to;
+  int rc;
+  if ((rc = make_rows_map(&tq, p->q, p->batch, p->seqlen_q, p->heads_q, DR, p->q_strides, a.group, tokens, kBf16)) ||
+      (rc = make_rows_map(&to, p->o, p->batch, p->seqlen_q, p->heads_q, DR, p->o_strides, a.group, tokens, kBf16)) ||
+      (rc = make_pool_map(&tk, p->cache.k, p->cache, p->cache.k_strides, p->heads_k, DR, a.box_rows, kBf16)) ||
+      (rc = make_pool_map(&tv, p->cache.v, p->cache, p->cache.v_strides, p->heads_k, DR, a.box_rows, kBf16)))
+    return rc;
+  if (!launch_with_smem<fmha::paged_many_kernel<D, DR, kBf16, kE4m3>>(dev, plan.blocks, T::kThreads, T::kSmemBytes, stream, tq,
+                                                                      tk, tv, to, a))
+    return FMHA_ERR_LAUNCH;
+  return launch_join<kBf16, DR, 256>(a, plan, stream);
 }
 
 // (a 32-bit grid of blocks of 256 threads, 8 or 16 of them a row)
@@ -352,33 +384,13 @@ int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspac
   if ((double)p->batch * p->heads_k * plan.blocks_per_entry * tiles >= 2147483648.0) return FMHA_ERR_TOO_LARGE;
   if (plan.bytes() > 0 && (workspace == nullptr || workspace_bytes < plan.bytes())) return FMHA_ERR_WORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (plan.kernel_rows > 0) {
-    FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format, {
-      constexpr int D = DR == 64 ? 64 : 128;
-      if (plan.kernel_rows == 16) return launch_few<D, DR, kBf16, kE4m3, 16>(p, plan, workspace, dev, s);
-      if (plan.kernel_rows == 32) return launch_few<D, DR, kBf16, kE4m3, 32>(p, plan, workspace, dev, s);
-      return launch_few<D, DR, kBf16, kE4m3, 64>(p, plan, workspace, dev, s);
-    })
-  }
-  fmha::PagedSimpleArgs a;
-  a.cache = device_cache(p->cache);
-  a.q = static_cast<const uint8_t*>(p->q);
-  a.o = static_cast<uint8_t*>(p->o);
-  a.lse = p->lse;
-  a.q_batch = p->q_strides.batch * 2, a.q_row = p->q_strides.row * 2, a.q_head = p->q_strides.head * 2;
-  a.o_batch = p->o_strides.batch * 2, a.o_row = p->o_strides.row * 2, a.o_head = p->o_strides.head * 2;
-  a.seqused_k = p->seqused_k;
-  a.seqused_q = p->seqused_q;
-  a.heads_q = p->heads_q;
-  a.group = p->heads_q / p->heads_k;
-  a.seqlen_q = p->seqlen_q;
-  a.causal = p->causal != 0;
-  a.scale = p->scale;
-  a.rows = (long long)p->batch * p->seqlen_q * p->heads_q;
-  const unsigned grid = (unsigned)((a.rows + 3) / 4);
-  FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format,
-                      fmha::paged_simple_kernel<DR, kBf16, kE4m3><<<grid, 128, 0, s>>>(a);)
-  return cudaGetLastError() == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
+  FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format, {
+    constexpr int D = DR == 64 ? 64 : 128;
+    if (plan.kernel_rows == 16) return launch_few<D, DR, kBf16, kE4m3, 16>(p, plan, workspace, dev, s);
+    if (plan.kernel_rows == 32) return launch_few<D, DR, kBf16, kE4m3, 32>(p, plan, workspace, dev, s);
+    if (plan.kernel_rows == 64) return launch_few<D, DR, kBf16, kE4m3, 64>(p, plan, workspace, dev, s);
+    return launch_many<D, DR, kBf16, kE4m3>(p, plan, workspace, dev, s);
+  })
 }
 
 }  // extern "C"

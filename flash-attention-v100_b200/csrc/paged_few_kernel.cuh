@@ -57,6 +57,7 @@ struct FewTraits {
   static constexpr int kThreads = kE4m3 ? 512 : 256;
   static constexpr int kSmemBytes =
       1024 + kStages * kTileBytes + kCodeStages * kCodeBytes + kQBufs * kQBytes + 2 * kPBytes;
+  static_assert(kSmemBytes <= 230400, "the rest of the 227 KB is for what is declared in the kernel");
   static constexpr int kTmemCols = !kE4m3 ? 4 * kRows : kRows == 64 ? 512 : 256;
   // 8-bit caches are multiplied in fp16 (see the converting warps)
   static constexpr uint32_t kIdescQK = umma_idesc_f16(128, kRows, 0, 0, kBf16 && !kE4m3);
@@ -114,7 +115,7 @@ __device__ __forceinline__ float warp_totals(float (&v)[N], int lane) {
 template <int D, int DR, bool kBf16, bool kE4m3, int kRows>
 __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThreads, 1)
     paged_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                     const __grid_constant__ CUtensorMap tm_v, const PagedParams p) {
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedParams p) {
   using T = FewTraits<D, DR, kBf16, kE4m3, kRows>;
   constexpr int kStages = T::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   // by (Q is three pieces ahead at most)
   __shared__ uint64_t bar_code_full[kE4m3 ? T::kCodeStages : 1], bar_code_empty[kE4m3 ? T::kCodeStages : 1];
   __shared__ uint64_t bar_kt_full[2], bar_kt_free[2];
-  __shared__ uint32_t code_scale[kE4m3 ? T::kCodeStages : 1][128];  // the aligned word around a row's byte
+  __shared__ __align__(16) uint32_t code_scale[kE4m3 ? T::kCodeStages : 1][128];  // the aligned word around a row's byte
   __shared__ uint8_t code_select[kE4m3 ? T::kCodeStages : 1][32];    // which byte of it, two bits for each of four rows
   __shared__ uint8_t k_scale[kE4m3 ? 4 : 1][128];
   __shared__ __align__(8) uint8_t v_bf16[kE4m3 ? kStages : 1][8];
@@ -220,34 +221,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     return it;
   };
 
-  // the scale byte of a row in a stage of codes
-  [[maybe_unused]] auto scale_byte = [&](uint32_t stage, int row) -> uint32_t {
-    return code_scale[stage][row] >> ((code_select[stage][row >> 2] >> (row % 4 * 2) & 3) * 8) & 0xffu;
-  };
-
-  // Pages of a piece's tiles, in parts of box_rows rows, 32 parts at a time, a lane each, and the next 32 while these are used:
-  // a lookup takes microseconds when all of HBM's rate is used.
-  const int subs = 128 / p.box_rows;
-  struct Pages {
-    int now, next;
-  };
-  // the table's entry for part 32 * batch + lane (not looked at before it is used)
-  auto lookup = [&](const PagedPiece& it, int batch) {
-    const int part = 32 * batch + lane, key = it.first * 128 + part * p.box_rows;
-    int entry = -1;
-    if (part < it.tiles * subs && key < it.sk) entry = cache_entry(p.cache, it.z, key);
-    return entry;
-  };
-  // the page of a part of tile j, j in ascending order (num_pages, outside the pool, where there is none)
-  auto page_of = [&](const PagedPiece& it, Pages& w, int j, int sub) {
-    if (j > 0 && j * subs % 32 == 0) {
-      w.now = w.next;
-      w.next = lookup(it, j * subs / 32 + 1);
-    }
-    const int page = __shfl_sync(0xffffffffu, w.now, (j * subs + sub) & 31);
-    return (unsigned)page < (unsigned)p.cache.num_pages ? page : p.cache.num_pages;
-  };
-
+  const PagedPages pages{p};
   if (warp == 6) {
     // =========================== source of pieces, K and V producer ===========================
     // A lane per box: 128 / box_rows parts of a tile, kBoxes column blocks of each (codes: one); lanes 0-15 K's, 16-31 V's.
@@ -258,7 +232,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     constexpr uint32_t kBytes = kE4m3 ? T::kCodeBytes : T::kTileBytes;
     const bool is_v = lane >= 16;
     const int sub = (lane & 15) / kCols, box = lane % kCols;
-    const bool mine = sub < subs;
+    const bool mine = sub < pages.parts();
     const uint32_t dst = (kE4m3 ? code_smem : ring_smem) + box * T::kBoxBytes + sub * p.box_rows * 128;
     const CUtensorMap* const tm = is_v ? &tm_v : &tm_k;
     uint64_t* const fulls = kE4m3 ? bar_code_full : bar_kv_full;
@@ -280,21 +254,20 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       return it;
     };
     PagedPiece it = next_item();
-    Pages pages;
-    pages.now = lookup(it, 0);
+    int first_pages = pages.lookup(it, 0);
     while (ok && it.id >= 0) {
       PagedPiece after = it;
-      int pages_after = 0;
-      pages.next = lookup(it, 1);
+      int first_pages_after = 0;
+      PagedPages::Window window{first_pages, pages.lookup(it, 1)};
 #pragma unroll 1
       for (int j = 0; ok && j < max(it.tiles, 1); ++j) {
         if (j + 2 >= it.tiles && after.id == it.id) {
           after = next_item();
-          pages_after = lookup(after, 0);
+          first_pages_after = pages.lookup(after, 0);
         }
         if (j >= it.tiles) break;  // (no tiles at all)
-        const int page = page_of(it, pages, j, sub);
-        const int row = cache_page_row(p.cache, it.first * 128 + (j * subs + sub) * p.box_rows);
+        int row;
+        const int page = pages.page_of(it, window, j, sub, row);
         // K's slot and V's, the one behind it
         const uint32_t slot_v = slot + 1 == kRing ? 0 : slot + 1, phase_v = slot + 1 == kRing ? phase ^ 1 : phase;
         ok = ok && rolled_wait_warp(smem_u32(&empties[slot]), phase, &abort_word, 3) &&
@@ -309,7 +282,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         slot = slot + 2 >= kRing ? slot + 2 - kRing : slot + 2;
       }
       it = after;
-      pages.now = pages_after;
+      first_pages = first_pages_after;
     }
   } else if (warp == 5) {
     // =========================== Q producer; scales of codes ===========================
@@ -320,8 +293,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       const PagedPiece it = take_item();
       if (it.id < 0) break;
       if (it.tiles == 0) continue;
-      [[maybe_unused]] Pages pages = {};
-      if constexpr (kE4m3) pages = {lookup(it, 0), lookup(it, 1)};
+      [[maybe_unused]] PagedPages::Window window = {};
+      if constexpr (kE4m3) window = {pages.lookup(it, 0), pages.lookup(it, 1)};
       const uint32_t b = used % T::kQBufs, round = used / T::kQBufs;
       if (round > 0 && !rolled_wait_warp(smem_u32(&bar_q_free[b]), (round - 1) & 1, &abort_word, 24)) break;
       if constexpr (kE4m3 && kBf16) {
@@ -368,42 +341,11 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       __syncwarp();
       ++used;
       if constexpr (kE4m3) {
-        // Four rows a lane, in one page; the copy is of words, each the one that a row's byte is in (a word that holds a
-        // byte of an allocation is in it).
-        const int sub = lane * 4 / p.box_rows, in_part = lane * 4 % p.box_rows;
         bool ok = true;
 #pragma unroll 1
-        for (int j = 0; j < it.tiles; ++j) {
-          const int page = page_of(it, pages, j, sub);
-          const long long row = cache_page_row(p.cache, it.first * 128 + (j * subs + sub) * p.box_rows) + in_part;
-#pragma unroll 1
-          for (int n = 0; n < 2; ++n) {
-            const PagePool& pool = n ? p.cache.v : p.cache.k;
-            const uint8_t* src = pool.scales + page * pool.scale_page + row * pool.scale_row + it.h * pool.scale_head;
-            ok = ok && rolled_wait_warp(smem_u32(&bar_code_empty[slot]), phase, &abort_word, 19);
-            if (!ok) break;
-            const uint32_t to = smem_u32(&code_scale[slot][lane * 4]);
-            uint32_t select = 0;
-            if (page < p.cache.num_pages) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i, src += pool.scale_row) {
-                const size_t at = reinterpret_cast<size_t>(src);
-                copy_async4(to + 4 * i, reinterpret_cast<const void*>(at & ~size_t(3)));
-                select |= (uint32_t)(at & 3) << (2 * i);
-              }
-            } else {
-              sts128(to, 127, 127, 127, 127);
-            }
-            code_select[slot][lane] = (uint8_t)select;
-            copy_async_arrive(smem_u32(&bar_code_full[slot]));
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bar_code_full[slot]));
-            if (++slot == (uint32_t)T::kCodeStages) {
-              slot = 0;
-              phase ^= 1;
-            }
-          }
-        }
+        for (int j = 0; ok && j < it.tiles; ++j)
+          ok = pages.copy_scales(it, window, j, code_scale[0], code_select[0], bar_code_full, bar_code_empty, T::kCodeStages, slot,
+                                 phase, &abort_word);
         if (!ok) break;
       }
     }
@@ -727,7 +669,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           if (!ok) break;
           tc_fence_after();
           const uint32_t src = code_smem + slot * T::kCodeBytes + tid * 128;
-          k_scale[n & 3][tid] = (uint8_t)scale_byte(slot, tid);
+          k_scale[n & 3][tid] = (uint8_t)staged_scale(code_scale[0], code_select[0], slot, tid);
   #pragma unroll 2
           for (int i = 0; i < T::kChunks; i += 2) {  // 32 elements, 16 columns of tensor memory
             uint32_t w[16];
@@ -768,43 +710,50 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
                rolled_wait_warp(smem_u32(&bar_kv_empty[slot]), (n / kStages & 1) ^ 1, &abort_word, 23);
           if (!ok) break;
           const int rows = it.sk - (it.first + j) * 128 - row0;  // of the 32 that exist
-          const uint32_t my_scale = lane < rows ? scale_byte(from, row0 + lane) : 127u;
+          const uint32_t my_scale = lane < rows ? staged_scale(code_scale[0], code_select[0], from, row0 + lane) : 127u;
           const uint32_t fits = __ballot_sync(0xffffffffu, my_scale >= 112 && my_scale <= 134);
+          // Four lanes have the four chunks of 16 codes that make a row of a box, and the eight lanes of a shared-memory
+          // phase rows r and r ^ 5: then neither their loads nor their stores, which are swizzled by the row, meet in a bank.
           const uint32_t from_smem = code_smem + from * T::kCodeBytes, to_smem = ring_smem + slot * T::kTileBytes;
-          const bool plain = fits == 0xffffffffu;
-          // (one warp per scheduler does this: what hides its latencies is the next chunks)
-#pragma unroll(T::kChunks == 8 ? 4 : T::kChunks / 2)
-          for (int i = 0; i < T::kChunks; ++i) {
-            const int idx = lane + 32 * i, r = idx / T::kChunks, chunk = idx % T::kChunks, row = row0 + r;
-            const float4 f = lds128(from_smem + row * 128 + ((chunk ^ (row & 7)) << 4));
-            const uint32_t exists = r < rows ? 0xffffffffu : 0u;
-            const uint32_t codes[4] = {__float_as_uint(f.x) & exists, __float_as_uint(f.y) & exists,
-                                       __float_as_uint(f.z) & exists, __float_as_uint(f.w) & exists};
-            const uint32_t byte = __shfl_sync(0xffffffffu, my_scale, r);
-            uint32_t w[8];
+          const int in8 = lane & 4 ? lane >> 3 ^ 5 : lane >> 3, quarter = lane & 3;
+          const uint32_t ld = row0 * 128 + in8 * 128 + ((quarter ^ in8) << 4), st = row0 * 128 + in8 * 128 + ((quarter * 2 ^ in8) << 4);
+#pragma unroll 2
+          for (int k = 0; k < 4; ++k) {  // rows 8 k to 8 k + 7 of the warp's 32
+            const uint32_t byte = __shfl_sync(0xffffffffu, my_scale, 8 * k + in8);
+            const uint32_t h = (byte == 112 ? 0x0200u : (byte - 112) << 10) * 0x10001u;  // 2^(byte - 127) in fp16, twice
+            const bool plain = (fits >> (k & 2) * 8 & 0xffffu) == 0xffffu;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              w[2 * u] = e4m3x2_to_half2(codes[u] & 0xffffu);
-              w[2 * u + 1] = e4m3x2_to_half2(codes[u] >> 16);
-            }
-            if (plain || (fits >> (r & 16) & 0xffffu) == 0xffffu) {
-              const uint32_t h = (byte == 112 ? 0x0200u : (byte - 112) << 10) * 0x10001u;  // 2^(byte - 127) in fp16, twice
+            for (int box = 0; box < T::kBoxes; ++box) {
+              if (DR == 96 && box == 1 && quarter >= 2) continue;
+              const float4 f = lds128(from_smem + k * 1024 + (ld ^ box * 64));
+              const uint32_t codes[4] = {__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w)};
+              uint32_t w[8];
 #pragma unroll
-              for (int u = 0; u < 8; ++u) w[u] = mul_half2(w[u], h);
-            } else {
-              const float s = scale_value(byte);
-#pragma unroll
-              for (int u = 0; u < 8; ++u) {
-                const float2 v = __half22float2(*reinterpret_cast<__half2*>(&w[u]));
-                w[u] = pack16x2<kBf16>(v.x * s, v.y * s);
+              for (int u = 0; u < 4; ++u) {
+                w[2 * u] = e4m3x2_to_half2(codes[u] & 0xffffu);
+                w[2 * u + 1] = e4m3x2_to_half2(codes[u] >> 16);
               }
+              if (plain) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) w[u] = mul_half2(w[u], h);
+              } else {
+                const float s = scale_value(byte);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                  const float2 v = __half22float2(*reinterpret_cast<__half2*>(&w[u]));
+                  w[u] = pack16x2<kBf16>(v.x * s, v.y * s);
+                }
+              }
+              const uint32_t to = to_smem + box * T::kBoxBytes + k * 1024 + st;
+              sts128(to, w[0], w[1], w[2], w[3]);
+              sts128(to ^ 16, w[4], w[5], w[6], w[7]);
             }
-            // (threads of the second box start with their second half: the two boxes have the same banks)
-            const bool swap = (chunk >> 2) != 0;
-            const uint32_t at16 = (((chunk & 3) * 2 + (swap ? 1 : 0)) ^ (row & 7)) << 4;
-            const uint32_t base = to_smem + (chunk >> 2) * T::kBoxBytes + row * 128;
-            sts128(base + at16, swap ? w[4] : w[0], swap ? w[5] : w[1], swap ? w[6] : w[2], swap ? w[7] : w[3]);
-            sts128(base + (at16 ^ 16), swap ? w[0] : w[4], swap ? w[1] : w[5], swap ? w[2] : w[6], swap ? w[3] : w[7]);
+          }
+          // rows behind the entry's end: zeros, whatever the page holds there
+          __syncwarp();
+          if (lane >= rows) {
+            for (int i = 0; i < 8 * T::kBoxes; ++i)
+              sts128(to_smem + (i >> 3) * T::kBoxBytes + (row0 + lane) * 128 + (i & 7) * 16, 0, 0, 0, 0);
           }
           if (lane < 2) v_bf16[slot][2 * (warp - 12) + lane] = (fits >> (16 * lane) & 0xffffu) != 0xffffu;
           fence_proxy_async_smem();

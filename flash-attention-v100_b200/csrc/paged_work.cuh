@@ -20,7 +20,9 @@ struct PagedParams {
   unsigned group_mul;     // r / group = (r * group_mul) >> 16 for r < 256
   int blocks_per_entry;   // blocks of new tokens
   int tokens_per_block;
-  int box_rows;           // rows of a K or V box: what divides both a page and a tile
+  int rows_per_tile;      // rows of a block that lie together in its partial rows: all (few rows), or each half (many)
+  int box_rows;           // rows of a K or V box: what divides both a page and a tile, 128 >> part_shift
+  int part_shift;
   int min_share;          // units a block has at least
   float scale_log2;       // |scale| * log2(e)
   int negate;             // scale < 0: the tensor cores form -Q K^T
@@ -44,6 +46,7 @@ struct PagedPiece {
   int first, tiles;  // KV tiles [first, first + tiles); tiles = 0: the item sees no key at all
   int slot;          // of its partial rows, -1: the piece is the whole item
   int sq, sk;        // the entry's lengths
+  int n0, n1;        // (many rows) of the tiles, those that the first and the second half of the block's rows see
 };
 
 __device__ __forceinline__ void paged_lengths(const PagedParams& p, int z, int& sq, int& sk) {
@@ -55,9 +58,10 @@ __device__ __forceinline__ int paged_last_key(const PagedParams& p, int i, int s
   if (i >= sq) return -1;
   return p.causal ? max(-1, sk - sq + i) : sk - 1;
 }
-__device__ __forceinline__ int paged_tiles(const PagedParams& p, int token0, int sq, int sk) {
+// KV tiles that `tokens` tokens from token0 on see
+__device__ __forceinline__ int paged_tiles(const PagedParams& p, int token0, int tokens, int sq, int sk) {
   if (token0 >= sq) return 0;
-  return (paged_last_key(p, min(token0 + p.tokens_per_block, sq) - 1, sq, sk) + 128) / 128;
+  return (paged_last_key(p, min(token0 + tokens, sq) - 1, sq, sk) + 128) / 128;
 }
 
 __device__ __forceinline__ int row_token(const PagedParams& p, int r) { return (int)((unsigned)r * p.group_mul >> 16); }
@@ -70,15 +74,14 @@ struct PagedWork {
   int sq, sk;
   int share;
 
-  // (calls, not inlined: they run once a piece, and the instruction cache is what the roles of a block share)
   __device__ __forceinline__ void enter_pair(const PagedParams& p) {
     z = pair / p.blocks_per_entry;
     token0 = (pair - z * p.blocks_per_entry) * p.tokens_per_block;
     paged_lengths(p, z, sq, sk);
-    tiles = paged_tiles(p, token0, sq, sk);
+    tiles = paged_tiles(p, token0, p.tokens_per_block, sq, sk);
   }
 
-  __device__ __noinline__ void start(const PagedParams& p, int block, int blocks) {
+  __device__ __forceinline__ void start(const PagedParams& p, int block, int blocks) {
     const int lane = threadIdx.x & 31;
     const int pairs = p.batch * p.blocks_per_entry;
     auto units = [&](int f) {
@@ -118,10 +121,9 @@ struct PagedWork {
     enter_pair(p);
   }
 
-  __device__ __noinline__ PagedPiece next(const PagedParams& p, int block) {
-    PagedPiece it;
+  __device__ __forceinline__ PagedPiece next(const PagedParams& p, int block) {
+    PagedPiece it = {};  // (the last one, which says that there is none, has no tiles for anybody)
     it.id = -1;
-    it.tiles = 0;
 #pragma unroll 1
     while (pos < end) {
       const int w = tiles + kItemCost;
@@ -145,6 +147,9 @@ struct PagedWork {
       it.slot = first == 0 && last == tiles ? -1 : 2 * block + (first > 0 ? 0 : 1);
       it.sq = sq;
       it.sk = sk;
+      const int half = p.tokens_per_block / 2;
+      it.n0 = max(0, min(it.tiles, paged_tiles(p, token0, half, sq, sk) - first));
+      it.n1 = max(0, min(it.tiles, paged_tiles(p, token0 + half, half, sq, sk) - first));
       if (first == 0 && (threadIdx.x & 31) == 0)
         p.item_blocks[it.id] = make_int2(u0 / share, tiles > 0 ? (u0 + tiles - 1) / share : u0 / share);
       break;
@@ -152,6 +157,77 @@ struct PagedWork {
     return it;
   }
 };
+
+// Pages of a piece's tiles, in parts of box_rows rows, 32 parts at a time, a lane each, and the next 32 while these are used:
+// a lookup takes microseconds when all of HBM's rate is used.  For a converged warp.
+struct PagedPages {
+  const PagedParams& p;
+  struct Window {
+    int now, next;
+  };
+  __device__ __forceinline__ int parts() const { return 1 << p.part_shift; }  // of a tile
+
+  // the table's entry for part 32 * batch + lane (not looked at before it is used)
+  __device__ __forceinline__ int lookup(const PagedPiece& it, int batch) const {
+    const int part = 32 * batch + (threadIdx.x & 31), key = it.first * 128 + part * p.box_rows;
+    int entry = -1;
+    if (part < it.tiles << p.part_shift && key < it.sk) entry = cache_entry(p.cache, it.z, key);
+    return entry;
+  }
+  // page and row of a part of tile j, j in ascending order (num_pages, outside the pool, where there is none)
+  __device__ __forceinline__ int page_of(const PagedPiece& it, Window& w, int j, int part, int& row) const {
+    const int first = j << p.part_shift;
+    if (j > 0 && (first & 31) == 0) {
+      w.now = w.next;
+      w.next = lookup(it, first / 32 + 1);
+    }
+    const int page = __shfl_sync(0xffffffffu, w.now, (first + part) & 31);
+    row = cache_page_row(p.cache, it.first * 128 + (first + part) * p.box_rows);
+    return (unsigned)page < (unsigned)p.cache.num_pages ? page : p.cache.num_pages;
+  }
+  // Scales of a tile's K and V rows into their stages of the ring of codes: four rows a lane, which lie in one page.  What is
+  // copied is words, each the one that a row's byte is in (a word that holds a byte of an allocation is in it), and beside
+  // them which of a word's bytes it is.
+  __device__ __forceinline__ bool copy_scales(const PagedPiece& it, Window& w, int j, uint32_t* words, uint8_t* selects,
+                                              uint64_t* full, uint64_t* empty, uint32_t stages, uint32_t& slot,
+                                              uint32_t& phase, volatile int* abort_word) const {
+    const int lane = threadIdx.x & 31;
+    int row;
+    const int page = page_of(it, w, j, lane >> (5 - p.part_shift), row);
+    row += lane * 4 & (p.box_rows - 1);
+#pragma unroll 1
+    for (int n = 0; n < 2; ++n) {
+      const PagePool& pool = n ? p.cache.v : p.cache.k;
+      const uint8_t* src = pool.scales + page * pool.scale_page + row * pool.scale_row + it.h * pool.scale_head;
+      if (!rolled_wait_warp(smem_u32(&empty[slot]), phase, abort_word, 19)) return false;
+      const uint32_t to = smem_u32(words + slot * 128 + lane * 4);
+      uint32_t select = 0;
+      if (page < p.cache.num_pages) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i, src += pool.scale_row) {
+          const size_t at = reinterpret_cast<size_t>(src);
+          copy_async4(to + 4 * i, reinterpret_cast<const void*>(at & ~size_t(3)));
+          select |= (uint32_t)(at & 3) << (2 * i);
+        }
+      } else {
+        sts128(to, 127, 127, 127, 127);
+      }
+      selects[slot * 32 + lane] = (uint8_t)select;
+      copy_async_arrive(smem_u32(&full[slot]));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&full[slot]));
+      if (++slot == stages) {
+        slot = 0;
+        phase ^= 1;
+      }
+    }
+    return true;
+  }
+};
+// the scale byte of a row in a stage
+__device__ __forceinline__ uint32_t staged_scale(const uint32_t* words, const uint8_t* selects, uint32_t stage, int row) {
+  return words[stage * 128 + row] >> ((selects[stage * 32 + (row >> 2)] >> (row % 4 * 2) & 3) * 8) & 0xffu;
+}
 
 // Joins the pieces of the items that were cut: a warp per row.  Every partial row is normalised by its own row
 // sum; its weight is exp(lse_part - lse).
@@ -168,14 +244,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, in
   if (blocks.x < 0 || blocks.x >= blocks.y || blocks.y >= blocks_of_grid) return;
   const int h = item % p.heads_k, pair = item / p.heads_k;
   const int z = pair / p.blocks_per_entry;
-  const int token_in_block = row_token(p, row);
-  const int token = pair % p.blocks_per_entry * p.tokens_per_block + token_in_block;
-  const int hq = h * p.group + row - token_in_block * p.group;
+  const int half = row >= p.rows_per_tile ? 1 : 0, in_tile = row - half * p.rows_per_tile, t = row_token(p, in_tile);
+  const int token = pair % p.blocks_per_entry * p.tokens_per_block + half * (p.rows_per_tile / p.group) + t;
+  const int hq = h * p.group + in_tile - t * p.group;
   if (token >= p.seqlen_q) return;
   // part i: of block blocks.x + i.  Lane i has the weight of part i (of 32 at a time), so that their rows are loaded
   // side by side: one after the other, 17 parts took 14 us.
   const int parts = blocks.y - blocks.x + 1;
-  auto part_at = [&](int i) { return (long long)(2 * (blocks.x + i) + (i == 0 ? 1 : 0)) * kRows + row; };
+  auto part_at = [&](int i) { return (long long)(2 * (blocks.x + i) + (i == 0 ? 1 : 0)) * kRows + half * 128 + in_tile; };
   // a part that is NaN makes the row NaN
   float mx = -CUDART_INF_F;
   for (int i = lane; i < parts; i += 32) mx = max_nan(mx, p.lse_part[part_at(i)]);
