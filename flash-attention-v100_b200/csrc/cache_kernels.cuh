@@ -98,37 +98,17 @@ struct CacheWriteArgs {
   const uint8_t *k, *v;                                   // 16-bit rows
   long long k_batch, k_row, k_head, v_batch, v_row, v_head;  // byte strides
   const int32_t *seqlens, *seqused;
-  int heads, seqlen;
-  long long rows;  // batch * seqlen * heads
+  int heads, batch;
+  int rows;  // of an entry: seqlen * heads
 };
 
-// New rows into their pages.  kLanes threads a row (8 elements each), K and V of the same row by the same threads, so
-// that two loads are in flight and the place is worked out once.  What bounds it is HBM for chunks of a prompt and
-// the launch for single tokens.
-template <int DR, bool kBf16, bool kE4m3>
-__global__ void __launch_bounds__(256) cache_write_kernel(const CacheWriteArgs a) {
-  constexpr int kLanes = DR == 64 ? 8 : 16;  // (96: four of sixteen idle)
-  const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / kLanes;
-  const int sub = threadIdx.x % kLanes;
-  if (r >= a.rows) return;  // (rows of a warp share a shuffle below: masked by groups of kLanes, which return together)
-  const int h = (int)(r % a.heads);
-  const long long zi = r / a.heads;
-  const int z = (int)(zi / a.seqlen), i = (int)(zi % a.seqlen);
-  if (a.seqused != nullptr && i >= __ldg(a.seqused + z)) return;
-  const long long t = (long long)__ldg(a.seqlens + z) + i;
-  if (t < 0 || t >= cache_capacity(a.cache)) return;
-  const int page = cache_page(a.cache, z, (int)t);
-  if (page < 0) return;
-  const int slot = cache_page_row(a.cache, (int)t);
-  const bool in_row = sub * 8 < DR;
-  uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  if (in_row) {
-    x[0] = __ldg(reinterpret_cast<const uint4*>(a.k + z * a.k_batch + i * a.k_row + h * a.k_head) + sub);
-    x[1] = __ldg(reinterpret_cast<const uint4*>(a.v + z * a.v_batch + i * a.v_row + h * a.v_head) + sub);
-  }
+// K's and V's row of a token, 8 elements a thread, to its place in the pools
+template <int DR, bool kBf16, bool kE4m3, int kLanes>
+__device__ __forceinline__ void write_row(const PagedCache& c, int page, int slot, int h, int sub, bool in_row,
+                                          const uint4 (&x)[2]) {
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
-    const PagePool& pool = n ? a.cache.v : a.cache.k;
+    const PagePool& pool = n ? c.v : c.k;
     uint8_t* dst = pool.rows + page * pool.page + slot * pool.row + h * pool.head;
     if constexpr (!kE4m3) {
       if (in_row) reinterpret_cast<uint4*>(dst)[sub] = x[n];
@@ -163,53 +143,91 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CacheWriteArgs a
   }
 }
 
+// New rows into their pages.  kLanes threads a row (8 elements each), K and V of the same row by the same threads, so
+// that two loads are in flight and the place is worked out once.  What bounds it is HBM for chunks of a prompt and
+// the launch for single tokens.
+template <int DR, bool kBf16, bool kE4m3>
+__global__ void __launch_bounds__(256) cache_write_kernel(const CacheWriteArgs a) {
+  constexpr int kLanes = DR == 64 ? 8 : 16;  // (96: four of sixteen idle)
+  const int r = (int)(blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes), sub = threadIdx.x % kLanes;
+  if (r >= a.rows) return;  // (the threads of a row share a shuffle below, and return together)
+  const int i = (int)((unsigned)r / (unsigned)a.heads), h = r - i * a.heads;
+  const bool in_row = sub * 8 < DR;
+#pragma unroll 1
+  for (int z = blockIdx.y; z < a.batch; z += gridDim.y) {
+    const long long t = (long long)__ldg(a.seqlens + z) + i;
+    if (a.seqused != nullptr && i >= __ldg(a.seqused + z)) continue;
+    if (t < 0 || t >= cache_capacity(a.cache)) continue;
+    // (the row is asked for before its place is known)
+    uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (in_row) {
+      x[0] = __ldg(reinterpret_cast<const uint4*>(a.k + z * a.k_batch + i * a.k_row + h * a.k_head) + sub);
+      x[1] = __ldg(reinterpret_cast<const uint4*>(a.v + z * a.v_batch + i * a.v_row + h * a.v_head) + sub);
+    }
+    const int page = cache_page(a.cache, z, (int)t);
+    if (page < 0) continue;
+    const int slot = cache_page_row(a.cache, (int)t);
+    write_row<DR, kBf16, kE4m3, kLanes>(a.cache, page, slot, h, sub, in_row, x);
+  }
+}
+
 struct CacheReadArgs {
   PagedCache cache;
   uint8_t *k, *v;
   long long k_batch, k_row, k_head, v_batch, v_row, v_head;  // byte strides
   const int32_t* seqused_k;
-  int heads, seqlen;
-  long long rows;  // batch * seqlen * heads
+  int heads, batch;
+  int rows;  // of an entry: seqlen * heads
 };
 
-// Rows out of their pages, zeros behind an entry's end.
+// Rows out of their pages, zeros behind an entry's end.  A thread has 16 elements of a row of K and of V.
 template <int DR, bool kBf16, bool kE4m3>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) {
-  constexpr int kLanes = DR / 8;
-  const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long r = n / kLanes;
-  const int sub = (int)(n % kLanes);
+  constexpr int kLanes = DR / 16;
+  const unsigned n = blockIdx.x * 256 + threadIdx.x;
+  const int r = (int)(n / kLanes), sub = (int)(n % kLanes);
   if (r >= a.rows) return;
-  const int h = (int)(r % a.heads);
-  const long long zi = r / a.heads;
-  const int z = (int)(zi / a.seqlen), t = (int)(zi % a.seqlen);
-  const int sk = min(__ldg(a.seqused_k + z), cache_capacity(a.cache));
-  const int page = t < sk ? cache_page(a.cache, z, t) : -1;
-  uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  if (page >= 0) {
-    const int slot = cache_page_row(a.cache, t);
-    const uint8_t* src[2];
-    float s[2];
+  const int t = (int)((unsigned)r / (unsigned)a.heads), h = r - t * a.heads;
+#pragma unroll 1
+  for (int z = blockIdx.y; z < a.batch; z += gridDim.y) {
+    const int sk = min(__ldg(a.seqused_k + z), cache_capacity(a.cache));
+    const int page = t < sk ? cache_page(a.cache, z, t) : -1;
+    uint4 x[2][2] = {};
+    if (page >= 0) {
+      const int slot = cache_page_row(a.cache, t);
+      uint32_t scale[2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const PagePool& pool = n ? a.cache.v : a.cache.k;
-      src[n] = pool.rows + page * pool.page + slot * pool.row + h * pool.head;
-      if constexpr (kE4m3)
-        s[n] = scale_value(__ldg(pool.scales + page * pool.scale_page + slot * pool.scale_row + h * pool.scale_head));
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < 2; ++n) {
+        const PagePool& pool = n ? a.cache.v : a.cache.k;
+        const uint4* src = reinterpret_cast<const uint4*>(pool.rows + page * pool.page + slot * pool.row + h * pool.head);
+        if constexpr (kE4m3) {
+          x[n][0] = __ldg(src + sub);
+          scale[n] = __ldg(pool.scales + page * pool.scale_page + slot * pool.scale_row + h * pool.scale_head);
+        } else {
+          x[n][0] = __ldg(src + 2 * sub);
+          x[n][1] = __ldg(src + 2 * sub + 1);
+        }
+      }
       if constexpr (kE4m3) {
-        const uint2 codes = __ldg(reinterpret_cast<const uint2*>(src[n]) + sub);
-        const uint2 lo = e4m3x4_to_16<kBf16>(codes.x, s[n]), hi = e4m3x4_to_16<kBf16>(codes.y, s[n]);
-        x[n] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      } else {
-        x[n] = __ldg(reinterpret_cast<const uint4*>(src[n]) + sub);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float s = scale_value(scale[n]);
+          const uint4 codes = x[n][0];
+          const uint2 w0 = e4m3x4_to_16<kBf16>(codes.x, s), w1 = e4m3x4_to_16<kBf16>(codes.y, s);
+          const uint2 w2 = e4m3x4_to_16<kBf16>(codes.z, s), w3 = e4m3x4_to_16<kBf16>(codes.w, s);
+          x[n][0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
+          x[n][1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
+        }
       }
     }
+    // (written once, read by somebody else: not to push the cache's lines out)
+    uint4* const k = reinterpret_cast<uint4*>(a.k + z * a.k_batch + t * a.k_row + h * a.k_head) + 2 * sub;
+    uint4* const v = reinterpret_cast<uint4*>(a.v + z * a.v_batch + t * a.v_row + h * a.v_head) + 2 * sub;
+    __stcs(k, x[0][0]);
+    __stcs(k + 1, x[0][1]);
+    __stcs(v, x[1][0]);
+    __stcs(v + 1, x[1][1]);
   }
-  reinterpret_cast<uint4*>(a.k + z * a.k_batch + t * a.k_row + h * a.k_head)[sub] = x[0];
-  reinterpret_cast<uint4*>(a.v + z * a.v_batch + t * a.v_row + h * a.v_head)[sub] = x[1];
 }
 
 }  // namespace fmha

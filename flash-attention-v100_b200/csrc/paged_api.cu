@@ -287,8 +287,13 @@ int launch_many(const FmhaPagedFwdParams* p, const PagedPlan& plan, void* worksp
   return launch_join<kBf16, DR, 256>(a, plan, stream);
 }
 
-// (a 32-bit grid of blocks of 256 threads, 8 or 16 of them a row)
-constexpr long long kMaxCacheRows = 1ll << 34;
+// rows of an entry (a thread's row is counted in 32 bits)
+constexpr long long kMaxCacheRows = 1ll << 27;
+
+// blocks of `per_block` rows for every entry
+dim3 cache_grid(int rows, int per_block, int batch) {
+  return dim3((unsigned)((rows + per_block - 1) / per_block), (unsigned)std::min(batch, 65535));
+}
 
 }  // namespace
 
@@ -300,9 +305,9 @@ int fmha_cache_write(const FmhaCacheWriteParams* p, void* stream) {
   if (rc) return rc;
   if (p->seqlen < 0) return FMHA_ERR_BAD_SHAPE;
   if ((rc = check_cache(p->cache, p->heads))) return rc;
-  const long long rows = (long long)p->batch * p->seqlen * p->heads;
-  if (rows == 0) return FMHA_OK;
-  if (rows > kMaxCacheRows) return FMHA_ERR_TOO_LARGE;
+  const long long rows = (long long)p->seqlen * p->heads;
+  if (rows == 0 || p->batch == 0) return FMHA_OK;
+  if (rows > kMaxCacheRows || rows * p->batch > (1ll << 34)) return FMHA_ERR_TOO_LARGE;
   if (p->k == nullptr || p->v == nullptr || p->seqlens == nullptr) return FMHA_ERR_NULL_POINTER;
   if (!aligned16(p->k) || !aligned16(p->v)) return FMHA_ERR_BAD_ALIGNMENT;
   if ((rc = check_strides(p->k_strides, p->seqlen, p->heads, p->batch))) return rc;
@@ -316,10 +321,9 @@ int fmha_cache_write(const FmhaCacheWriteParams* p, void* stream) {
   a.seqlens = p->seqlens;
   a.seqused = p->seqused;
   a.heads = p->heads;
-  a.seqlen = p->seqlen;
-  a.rows = rows;
-  const int per_block = 256 / (p->head_dim == 64 ? 8 : 16);
-  const unsigned grid = (unsigned)((rows + per_block - 1) / per_block);
+  a.batch = p->batch;
+  a.rows = (int)rows;
+  const dim3 grid = cache_grid(a.rows, 256 / (p->head_dim == 64 ? 8 : 16), p->batch);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format,
                       fmha::cache_write_kernel<DR, kBf16, kE4m3><<<grid, 256, 0, s>>>(a);)
@@ -332,9 +336,9 @@ int fmha_cache_read(const FmhaCacheReadParams* p, void* stream) {
   if (rc) return rc;
   if (p->seqlen < 0) return FMHA_ERR_BAD_SHAPE;
   if ((rc = check_cache(p->cache, p->heads))) return rc;
-  const long long rows = (long long)p->batch * p->seqlen * p->heads;
-  if (rows == 0) return FMHA_OK;
-  if (rows > kMaxCacheRows) return FMHA_ERR_TOO_LARGE;
+  const long long rows = (long long)p->seqlen * p->heads;
+  if (rows == 0 || p->batch == 0) return FMHA_OK;
+  if (rows > kMaxCacheRows || rows * p->batch > (1ll << 34)) return FMHA_ERR_TOO_LARGE;
   if (p->k == nullptr || p->v == nullptr || p->seqused_k == nullptr) return FMHA_ERR_NULL_POINTER;
   if (!aligned16(p->k) || !aligned16(p->v)) return FMHA_ERR_BAD_ALIGNMENT;
   if ((rc = check_strides(p->k_strides, p->seqlen, p->heads, p->batch))) return rc;
@@ -347,9 +351,9 @@ int fmha_cache_read(const FmhaCacheReadParams* p, void* stream) {
   a.v_batch = p->v_strides.batch * 2, a.v_row = p->v_strides.row * 2, a.v_head = p->v_strides.head * 2;
   a.seqused_k = p->seqused_k;
   a.heads = p->heads;
-  a.seqlen = p->seqlen;
-  a.rows = rows;
-  const unsigned grid = (unsigned)((rows * (p->head_dim / 8) + 255) / 256);
+  a.batch = p->batch;
+  a.rows = (int)rows;
+  const dim3 grid((unsigned)((rows * (p->head_dim / 16) + 255) / 256), (unsigned)std::min(p->batch, 65535));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format,
                       fmha::cache_read_kernel<DR, kBf16, kE4m3><<<grid, 256, 0, s>>>(a);)

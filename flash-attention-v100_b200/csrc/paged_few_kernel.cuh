@@ -187,6 +187,22 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     }
     fence_barrier_init();
   }
+  // The first piece and its pages are worked out beside the rest of the set-up (2 us of loads that depend on one another).
+  const PagedPages pages{p};
+  PagedWork work;
+  PagedPiece first_piece = {};
+  int first_pages = -1;
+  if (warp == 6) {
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      tma_prefetch_desc(&tm_q);
+    }
+    __syncwarp();
+    work.start(p, blockIdx.x, gridDim.x);
+    first_piece = work.next(p, blockIdx.x);
+    first_pages = pages.lookup(first_piece, 0);
+  }
   if (warp == 4) {
     tmem_alloc(smem_u32(&tmem_base_slot), T::kTmemCols);
     tmem_relinquish();
@@ -202,6 +218,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
+  grid_dependents_may_start();  // the joining kernel, which then need not be launched when this one ends
 
   uint32_t item_cnt = 0;
   auto take_item = [&]() -> PagedPiece {
@@ -221,7 +238,6 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     return it;
   };
 
-  const PagedPages pages{p};
   if (warp == 6) {
     // =========================== source of pieces, K and V producer ===========================
     // A lane per box: 128 / box_rows parts of a tile, kBoxes column blocks of each (codes: one); lanes 0-15 K's, 16-31 V's.
@@ -237,12 +253,10 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     const CUtensorMap* const tm = is_v ? &tm_v : &tm_k;
     uint64_t* const fulls = kE4m3 ? bar_code_full : bar_kv_full;
     uint64_t* const empties = kE4m3 ? bar_code_empty : bar_kv_empty;
-    PagedWork work;
-    work.start(p, blockIdx.x, gridDim.x);
     bool ok = true;
     uint32_t slot = 0, phase = 1, published = 0;
     auto next_item = [&]() -> PagedPiece {
-      PagedPiece it = work.next(p, blockIdx.x);
+      const PagedPiece it = published == 0 ? first_piece : work.next(p, blockIdx.x);
       const uint32_t s = published % T::kItemStages, round = published / T::kItemStages;
       if (round > 0) ok = rolled_wait_warp(smem_u32(&bar_item_empty[s]), (round - 1) & 1, &abort_word, 2);
       if (ok && lane == 0) {
@@ -254,7 +268,6 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       return it;
     };
     PagedPiece it = next_item();
-    int first_pages = pages.lookup(it, 0);
     while (ok && it.id >= 0) {
       PagedPiece after = it;
       int first_pages_after = 0;

@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(ManyTraits<D, DR, kBf16, kE4m3>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
+  grid_dependents_may_start();  // the joining kernel (see paged_few_kernel.cuh)
 
   uint32_t item_cnt = 0;
   auto take_item = [&]() -> PagedPiece {

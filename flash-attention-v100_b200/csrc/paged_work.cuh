@@ -248,44 +248,57 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, in
   const int token = pair % p.blocks_per_entry * p.tokens_per_block + half * (p.rows_per_tile / p.group) + t;
   const int hq = h * p.group + in_tile - t * p.group;
   if (token >= p.seqlen_q) return;
-  // part i: of block blocks.x + i.  Lane i has the weight of part i (of 32 at a time), so that their rows are loaded
-  // side by side: one after the other, 17 parts took 14 us.
+  // part i: of block blocks.x + i.  Lane i has the weight of part i (of 32 at a time); rows are asked for eight at a time,
+  // and before the weights are there: one after the other, 17 parts took 14 us.
   const int parts = blocks.y - blocks.x + 1;
   auto part_at = [&](int i) { return (long long)(2 * (blocks.x + i) + (i == 0 ? 1 : 0)) * kRows + half * 128 + in_tile; };
-  // a part that is NaN makes the row NaN
-  float mx = -CUDART_INF_F;
-  for (int i = lane; i < parts; i += 32) mx = max_nan(mx, p.lse_part[part_at(i)]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-  const float base = mx == -CUDART_INF_F ? 0.f : mx;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
+  float sum = 0.f, base = -CUDART_INF_F;
   const int col = lane * 4;
+#pragma unroll 1
   for (int i0 = 0; i0 < parts; i0 += 32) {
     const float lp = i0 + lane < parts ? p.lse_part[part_at(i0 + lane)] : -CUDART_INF_F;
-    // nothing visible in this part (-inf): its weight is 0, and its row is not read; (inf - inf would be NaN)
+    float4 v[2][8];
+    auto ask = [&](int buf, int i1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[buf][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i1 + i < 32 && i0 + i1 + i < parts && col < DR)
+          v[buf][i] = *reinterpret_cast<const float4*>(p.o_part + part_at(i0 + i1 + i) * DR + col);
+      }
+    };
+    ask(0, 0);
+    ask(1, 8);
+    // a part that is NaN makes the row NaN
+    float mx = max_nan(lp, base);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    if (mx != base && base != -CUDART_INF_F) {  // more than 32 parts, and a larger one among the later ones
+      const float a = expf(base - mx);
+      sum *= a;
+      acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
+    }
+    base = mx;
+    // nothing visible in a part (-inf): its weight is 0, and its row may be anything; (inf - inf would be NaN)
     const float mine = lp == -CUDART_INF_F ? 0.f : lp == base ? 1.f : expf(lp - base);
-#pragma unroll 1
-    for (int i1 = 0; i1 < 32 && i0 + i1 < parts; i1 += 8) {
-      float4 v[8];
-      float w[8];
+#pragma unroll
+    for (int i1 = 0; i1 < 32; i1 += 8) {
+      if (i0 + i1 >= parts) break;
+      float4(&x)[8] = v[i1 / 8 % 2];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        w[i] = __shfl_sync(0xffffffffu, mine, i1 + i);
-        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (w[i] != 0.f && col < DR) v[i] = *reinterpret_cast<const float4*>(p.o_part + part_at(i0 + i1 + i) * DR + col);
+        const float w = __shfl_sync(0xffffffffu, mine, i1 + i);
+        if (w != 0.f) {
+          sum += w;
+          acc.x += w * x[i].x, acc.y += w * x[i].y, acc.z += w * x[i].z, acc.w += w * x[i].w;
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum += w[i];
-        acc.x += w[i] * v[i].x, acc.y += w[i] * v[i].y, acc.z += w[i] * v[i].z, acc.w += w[i] * v[i].w;
-      }
+      if (i1 < 16) ask(i1 / 8 % 2, i1 + 16);
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (lane == 0)
-    p.lse[((long long)z * p.heads_k * p.group + hq) * p.seqlen_q + token] =
-        sum == 0.f ? -CUDART_INF_F : base + logf(sum);
+    p.lse[((long long)z * p.heads_k * p.group + hq) * p.seqlen_q + token] = sum == 0.f ? -CUDART_INF_F : base + logf(sum);
   if (col < DR) {
     constexpr bool kBf16 = std::is_same<E, __nv_bfloat16>::value;
     uint2 v;

@@ -438,6 +438,10 @@ __device__ __forceinline__ int clc_answer(uint32_t answer_smem) {
 // In a kernel that the launch allows to start early: the kernels before it are done, their writes visible
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// The kernel launched behind this one may be scheduled as soon as every block has said so (what it needs of this one it waits
+// for with grid_dependency_wait)
+__device__ __forceinline__ void grid_dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // warpgroup-wide register re-budgeting: every warp of an aligned group of 4 warps executes it
 template <int N>
 __device__ __forceinline__ void reg_alloc() {
