@@ -114,28 +114,36 @@ __device__ __forceinline__ void write_row(const PagedCache& c, int page, int slo
       if (in_row) reinterpret_cast<uint4*>(dst)[sub] = x[n];
     } else {
       using E = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
-      float f[8];
-      unpack8<E>(x[n], f);
-      float top = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (!isfinite(f[j])) f[j] = CUDART_NAN_F;
-        top = fmaxf(top, fabsf(f[j]));  // (a NaN operand leaves the other)
-      }
+      // The largest magnitude by its bits, whose order is the values' (infinity and NaN above all others)
+      constexpr uint32_t kAbs = 0x7fff7fffu, kInfinity = kBf16 ? 0x7f80u : 0x7c00u;
+      const uint32_t m2 = __vmaxu2(__vmaxu2(x[n].x & kAbs, x[n].y & kAbs), __vmaxu2(x[n].z & kAbs, x[n].w & kAbs));
+      uint32_t m = max(m2 >> 16, m2 & 0xffffu);
       const uint32_t group = (kLanes == 8 ? 0xffu : 0xffffu) << (threadIdx.x % 32 / kLanes * kLanes);
 #pragma unroll
-      for (int off = kLanes / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(group, top, off));
-      const int e = scale_exponent<kBf16>(top);
+      for (int off = kLanes / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(group, m, off));
+      float f[8];
+      unpack8<E>(x[n], f);
+      if (m >= kInfinity) {  // rare: what is not finite becomes NaN, and the scale is the others'
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (!isfinite(f[j])) f[j] = CUDART_NAN_F;
+          top = fmaxf(top, fabsf(f[j]));  // (a NaN operand leaves the other)
+        }
+#pragma unroll
+        for (int off = kLanes / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(group, top, off));
+        m = kBf16 ? __float_as_uint(top) >> 16 : (uint32_t)__half_as_ushort(__float2half_rn(top));
+      }
+      const int e = scale_exponent<kBf16>(kBf16 ? __uint_as_float(m << 16) : __half2float(__ushort_as_half((unsigned short)m)));
       const float s = exp2_neg_int(e), most = code_limit<kBf16>(e);
+      if (most < 448.f) {  // rare, too
+#pragma unroll
+        for (int j = 0; j < 8; ++j)  // (minimum and maximum would drop a NaN)
+          if (fabsf(f[j] * s) > most) f[j] = copysignf(most / s, f[j]);
+      }
       uint32_t w[2] = {0, 0};
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        // minimum and maximum would drop a NaN: the limits are applied to what is one of the numbers
-        float lo = f[j] * s, hi = f[j + 1] * s;
-        lo = fabsf(lo) > most ? copysignf(most, lo) : lo;
-        hi = fabsf(hi) > most ? copysignf(most, hi) : hi;
-        w[j / 4] |= float2_to_e4m3x2(lo, hi) << (j % 4 * 8);
-      }
+      for (int j = 0; j < 8; j += 2) w[j / 4] |= float2_to_e4m3x2(f[j] * s, f[j + 1] * s) << (j % 4 * 8);
       if (in_row) reinterpret_cast<uint2*>(dst)[sub] = make_uint2(w[0], w[1]);
       if (sub == 0)
         pool.scales[page * pool.scale_page + slot * pool.scale_row + h * pool.scale_head] = (uint8_t)(e + 127);
@@ -143,31 +151,44 @@ __device__ __forceinline__ void write_row(const PagedCache& c, int page, int slo
   }
 }
 
+// Rows that a thread of either kernel has: what bounds them is the chain of loads from an entry's length by its table to
+// the row's place, and more rows side by side hide it.  One row / four, us: four chunks of up to 4096 tokens into an 8-bit cache
+// WRITE_ONE / WRITE_FOUR, eight conversations of 1024 to 8192 tokens out of one READ_ONE / READ_FOUR.
+constexpr int kCacheRows = 4;
+
 // New rows into their pages.  kLanes threads a row (8 elements each), K and V of the same row by the same threads, so
-// that two loads are in flight and the place is worked out once.  What bounds it is HBM for chunks of a prompt and
-// the launch for single tokens.
+// that the place is worked out once.
 template <int DR, bool kBf16, bool kE4m3>
 __global__ void __launch_bounds__(256) cache_write_kernel(const CacheWriteArgs a) {
   constexpr int kLanes = DR == 64 ? 8 : 16;  // (96: four of sixteen idle)
-  const int r = (int)(blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes), sub = threadIdx.x % kLanes;
-  if (r >= a.rows) return;  // (the threads of a row share a shuffle below, and return together)
-  const int i = (int)((unsigned)r / (unsigned)a.heads), h = r - i * a.heads;
+  constexpr int kStep = 256 / kLanes;
+  const int r0 = (int)(blockIdx.x * (kStep * kCacheRows) + threadIdx.x / kLanes), sub = threadIdx.x % kLanes;
   const bool in_row = sub * 8 < DR;
 #pragma unroll 1
   for (int z = blockIdx.y; z < a.batch; z += gridDim.y) {
-    const long long t = (long long)__ldg(a.seqlens + z) + i;
-    if (a.seqused != nullptr && i >= __ldg(a.seqused + z)) continue;
-    if (t < 0 || t >= cache_capacity(a.cache)) continue;
-    // (the row is asked for before its place is known)
-    uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    if (in_row) {
-      x[0] = __ldg(reinterpret_cast<const uint4*>(a.k + z * a.k_batch + i * a.k_row + h * a.k_head) + sub);
-      x[1] = __ldg(reinterpret_cast<const uint4*>(a.v + z * a.v_batch + i * a.v_row + h * a.v_head) + sub);
+    const int held = __ldg(a.seqlens + z), used = a.seqused == nullptr ? 0x7fffffff : __ldg(a.seqused + z);
+    uint4 x[kCacheRows][2];
+    int page[kCacheRows];
+#pragma unroll
+    for (int k = 0; k < kCacheRows; ++k) {
+      const int r = r0 + k * kStep, i = (int)((unsigned)r / (unsigned)a.heads), h = r - i * a.heads;
+      const long long t = (long long)held + i;
+      x[k][0] = x[k][1] = make_uint4(0, 0, 0, 0);
+      page[k] = -1;
+      if (r < a.rows && i < used && t >= 0 && t < cache_capacity(a.cache)) {
+        page[k] = cache_entry(a.cache, z, (int)t);
+        if (in_row) {
+          x[k][0] = __ldg(reinterpret_cast<const uint4*>(a.k + z * a.k_batch + i * a.k_row + h * a.k_head) + sub);
+          x[k][1] = __ldg(reinterpret_cast<const uint4*>(a.v + z * a.v_batch + i * a.v_row + h * a.v_head) + sub);
+        }
+      }
     }
-    const int page = cache_page(a.cache, z, (int)t);
-    if (page < 0) continue;
-    const int slot = cache_page_row(a.cache, (int)t);
-    write_row<DR, kBf16, kE4m3, kLanes>(a.cache, page, slot, h, sub, in_row, x);
+#pragma unroll
+    for (int k = 0; k < kCacheRows; ++k) {
+      if ((unsigned)page[k] >= (unsigned)a.cache.num_pages) continue;  // (the threads of a row share a shuffle, and skip it together)
+      const int r = r0 + k * kStep, i = (int)((unsigned)r / (unsigned)a.heads), h = r - i * a.heads;
+      write_row<DR, kBf16, kE4m3, kLanes>(a.cache, page[k], cache_page_row(a.cache, held + i), h, sub, in_row, x[k]);
+    }
   }
 }
 
@@ -180,53 +201,60 @@ struct CacheReadArgs {
   int rows;  // of an entry: seqlen * heads
 };
 
-// Rows out of their pages, zeros behind an entry's end.  A thread has 16 elements of a row of K and of V.
+// Rows out of their pages, zeros behind an entry's end.  A thread has 8 elements of a row of K and of V.
 template <int DR, bool kBf16, bool kE4m3>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) {
-  constexpr int kLanes = DR / 16;
-  const unsigned n = blockIdx.x * 256 + threadIdx.x;
-  const int r = (int)(n / kLanes), sub = (int)(n % kLanes);
-  if (r >= a.rows) return;
-  const int t = (int)((unsigned)r / (unsigned)a.heads), h = r - t * a.heads;
+  constexpr unsigned kLanes = DR / 8, kBlockRows = 256 / kLanes;  // (96: 4 of 256 threads idle)
+  const int in_block = (int)(threadIdx.x / kLanes), sub = (int)(threadIdx.x % kLanes);
+  if (in_block >= (int)kBlockRows) return;
+  const int r0 = (int)(blockIdx.x * (kBlockRows * kCacheRows)) + in_block;
 #pragma unroll 1
   for (int z = blockIdx.y; z < a.batch; z += gridDim.y) {
     const int sk = min(__ldg(a.seqused_k + z), cache_capacity(a.cache));
-    const int page = t < sk ? cache_page(a.cache, z, t) : -1;
-    uint4 x[2][2] = {};
-    if (page >= 0) {
+    int page[kCacheRows];
+#pragma unroll
+    for (int k = 0; k < kCacheRows; ++k) {
+      const int r = r0 + k * (int)kBlockRows, t = (int)((unsigned)r / (unsigned)a.heads);
+      page[k] = -1;
+      if (r < a.rows && t < sk) page[k] = cache_entry(a.cache, z, t);
+    }
+    uint4 x[kCacheRows][2] = {};
+    uint32_t scale[kCacheRows][2] = {};
+#pragma unroll
+    for (int k = 0; k < kCacheRows; ++k) {
+      if ((unsigned)page[k] >= (unsigned)a.cache.num_pages) continue;
+      const int r = r0 + k * (int)kBlockRows, t = (int)((unsigned)r / (unsigned)a.heads), h = r - t * a.heads;
       const int slot = cache_page_row(a.cache, t);
-      uint32_t scale[2];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const PagePool& pool = n ? a.cache.v : a.cache.k;
-        const uint4* src = reinterpret_cast<const uint4*>(pool.rows + page * pool.page + slot * pool.row + h * pool.head);
+        const uint8_t* src = pool.rows + page[k] * pool.page + slot * pool.row + h * pool.head;
         if constexpr (kE4m3) {
-          x[n][0] = __ldg(src + sub);
-          scale[n] = __ldg(pool.scales + page * pool.scale_page + slot * pool.scale_row + h * pool.scale_head);
+          const uint2 codes = __ldg(reinterpret_cast<const uint2*>(src) + sub);
+          x[k][n].x = codes.x;
+          x[k][n].y = codes.y;
+          scale[k][n] = __ldg(pool.scales + page[k] * pool.scale_page + slot * pool.scale_row + h * pool.scale_head);
         } else {
-          x[n][0] = __ldg(src + 2 * sub);
-          x[n][1] = __ldg(src + 2 * sub + 1);
-        }
-      }
-      if constexpr (kE4m3) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float s = scale_value(scale[n]);
-          const uint4 codes = x[n][0];
-          const uint2 w0 = e4m3x4_to_16<kBf16>(codes.x, s), w1 = e4m3x4_to_16<kBf16>(codes.y, s);
-          const uint2 w2 = e4m3x4_to_16<kBf16>(codes.z, s), w3 = e4m3x4_to_16<kBf16>(codes.w, s);
-          x[n][0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
-          x[n][1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
+          x[k][n] = __ldg(reinterpret_cast<const uint4*>(src) + sub);
         }
       }
     }
-    // (written once, read by somebody else: not to push the cache's lines out)
-    uint4* const k = reinterpret_cast<uint4*>(a.k + z * a.k_batch + t * a.k_row + h * a.k_head) + 2 * sub;
-    uint4* const v = reinterpret_cast<uint4*>(a.v + z * a.v_batch + t * a.v_row + h * a.v_head) + 2 * sub;
-    __stcs(k, x[0][0]);
-    __stcs(k + 1, x[0][1]);
-    __stcs(v, x[1][0]);
-    __stcs(v + 1, x[1][1]);
+#pragma unroll
+    for (int k = 0; k < kCacheRows; ++k) {
+      const int r = r0 + k * (int)kBlockRows, t = (int)((unsigned)r / (unsigned)a.heads), h = r - t * a.heads;
+      if (r >= a.rows) break;
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float s = scale_value(scale[k][n]);
+          const uint2 lo = e4m3x4_to_16<kBf16>(x[k][n].x, s), hi = e4m3x4_to_16<kBf16>(x[k][n].y, s);
+          x[k][n] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+      }
+      // (written once, read by somebody else: not to push the cache's lines out)
+      __stcs(reinterpret_cast<uint4*>(a.k + z * a.k_batch + t * a.k_row + h * a.k_head) + sub, x[k][0]);
+      __stcs(reinterpret_cast<uint4*>(a.v + z * a.v_batch + t * a.v_row + h * a.v_head) + sub, x[k][1]);
+    }
   }
 }
 
