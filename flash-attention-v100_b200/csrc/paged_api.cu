@@ -304,9 +304,9 @@ int fmha_cache_write(const FmhaCacheWriteParams* p, void* stream) {
   int rc = check_sizes(p->batch, p->heads, p->head_dim, p->dtype);
   if (rc) return rc;
   if (p->seqlen < 0) return FMHA_ERR_BAD_SHAPE;
+  if (p->seqlen == 0 || p->batch == 0) return FMHA_OK;  // (empty tensors have no memory)
   if ((rc = check_cache(p->cache, p->heads))) return rc;
   const long long rows = (long long)p->seqlen * p->heads;
-  if (rows == 0 || p->batch == 0) return FMHA_OK;
   if (rows > kMaxCacheRows || rows * p->batch > (1ll << 34)) return FMHA_ERR_TOO_LARGE;
   if (p->k == nullptr || p->v == nullptr || p->seqlens == nullptr) return FMHA_ERR_NULL_POINTER;
   if (!aligned16(p->k) || !aligned16(p->v)) return FMHA_ERR_BAD_ALIGNMENT;
@@ -335,9 +335,9 @@ int fmha_cache_read(const FmhaCacheReadParams* p, void* stream) {
   int rc = check_sizes(p->batch, p->heads, p->head_dim, p->dtype);
   if (rc) return rc;
   if (p->seqlen < 0) return FMHA_ERR_BAD_SHAPE;
+  if (p->seqlen == 0 || p->batch == 0) return FMHA_OK;  // (empty tensors have no memory)
   if ((rc = check_cache(p->cache, p->heads))) return rc;
   const long long rows = (long long)p->seqlen * p->heads;
-  if (rows == 0 || p->batch == 0) return FMHA_OK;
   if (rows > kMaxCacheRows || rows * p->batch > (1ll << 34)) return FMHA_ERR_TOO_LARGE;
   if (p->k == nullptr || p->v == nullptr || p->seqused_k == nullptr) return FMHA_ERR_NULL_POINTER;
   if (!aligned16(p->k) || !aligned16(p->v)) return FMHA_ERR_BAD_ALIGNMENT;
@@ -373,8 +373,8 @@ int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspac
   if (p->heads_q <= 0 || p->heads_q % p->heads_k != 0 || p->heads_q / p->heads_k > 128 || p->seqlen_q < 0 ||
       !std::isfinite(p->scale) || p->scale == 0.f)
     return FMHA_ERR_BAD_SHAPE;
-  if ((rc = check_cache(p->cache, p->heads_k))) return rc;
   if (p->batch == 0 || p->seqlen_q == 0) return FMHA_OK;
+  if ((rc = check_cache(p->cache, p->heads_k))) return rc;
   if ((long long)p->seqlen_q * p->heads_q >= (1ll << 31) ||
       (long long)p->batch * p->heads_q * (p->seqlen_q / 128 + 2ll) >= (1ll << 31)) return FMHA_ERR_TOO_LARGE;
   if (p->q == nullptr || p->o == nullptr || p->lse == nullptr || p->seqused_k == nullptr) return FMHA_ERR_NULL_POINTER;
