@@ -16,7 +16,7 @@
 //   warp 6      source of pieces; TMA producer of K and V, a box per page (or per part of one)
 // 8-bit caches, whose codes and scales arrive in a ring of their own:
 //   warps 8-11  K: codes -> fp16, into tensor memory (a thread has a key there, as in the softmax)
-//   warps 12-15 V: codes times scale -> 16 bits, into the ring that 16-bit caches load directly
+//   warps 12 up V: codes times scale -> 16 bits, into the ring that 16-bit caches load directly
 //
 // Shared memory, 128-byte swizzle: ring of K and V tiles (128 x D, boxes of 64 columns; 8-bit caches: of V tiles), Q (kRows
 // x D, the same boxes), P^T (kRows x 128 keys, two boxes of 64 keys), codes (128 rows of 128 bytes).  Rows of V behind
@@ -54,7 +54,9 @@ struct FewTraits {
   static constexpr int kCodeBytes = 128 * 128;
   static constexpr int kQBufs = D == 128 && (kRows == 64 || (kE4m3 && kRows == 32)) ? 1 : 2;
   static constexpr int kItemStages = 8;
-  static constexpr int kThreads = kE4m3 ? 512 : 256;
+  // warps that convert V: as many as the registers of the softmax's row sums leave room for
+  static constexpr int kVWarps = kRows == 16 ? 8 : 4, kVRows = 128 / kVWarps;
+  static constexpr int kThreads = kE4m3 ? 32 * (12 + kVWarps) : 256;
   static constexpr int kSmemBytes =
       1024 + kStages * kTileBytes + kCodeStages * kCodeBytes + kQBufs * kQBytes + 2 * kPBytes;
   static_assert(kSmemBytes <= 230400, "the rest of the 227 KB is for what is declared in the kernel");
@@ -163,15 +165,15 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   if (threadIdx.x == 0) {
     for (int s = 0; s < T::kItemStages; ++s) {
       mbar_init(smem_u32(&bar_item_full[s]), 1);
-      mbar_init(smem_u32(&bar_item_empty[s]), kE4m3 ? 15 : 7);  // two MMA, Q, four softmax (eight converting) warps
+      mbar_init(smem_u32(&bar_item_empty[s]), kE4m3 ? 11 + T::kVWarps : 7);  // two MMA, Q, four softmax (eight converting) warps
     }
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&bar_kv_full[s]), kE4m3 ? 4 : 1);
+      mbar_init(smem_u32(&bar_kv_full[s]), kE4m3 ? T::kVWarps : 1);
       mbar_init(smem_u32(&bar_kv_empty[s]), 1);
     }
     for (int s = 0; s < T::kCodeStages; ++s) {
       mbar_init(smem_u32(&bar_code_full[s]), 34);  // TMA's thread, a warp's copies of scales, its word on which byte
-      mbar_init(smem_u32(&bar_code_empty[s]), 4);
+      mbar_init(smem_u32(&bar_code_empty[s]), s & 1 ? T::kVWarps : 4);  // (K has the even stages, V the odd ones)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&bar_q_full[b]), 1);
@@ -709,8 +711,9 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       }
     } else if (warp >= 12) {
       // =========================== V: codes times scale -> 16 bits in the ring ===========================
-      // A warp has 32 rows, that is two steps of O^T += V^T P^T.
-      const int row0 = 32 * (warp - 12);
+      // A warp has 16 or 32 rows, that is one or two steps of O^T += V^T P^T.
+      static_assert(T::kCodeStages % 2 == 0, "K has the even stages, V the odd ones");
+      const int row0 = T::kVRows * (warp - 12);
       uint32_t n = 0;
       bool ok = true;
       while (ok) {
@@ -722,7 +725,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           ok = rolled_wait_warp(smem_u32(&bar_code_full[from]), at / T::kCodeStages & 1, &abort_word, 22) &&
                rolled_wait_warp(smem_u32(&bar_kv_empty[slot]), (n / kStages & 1) ^ 1, &abort_word, 23);
           if (!ok) break;
-          const int rows = it.sk - (it.first + j) * 128 - row0;  // of the 32 that exist
+          const int rows = min(T::kVRows, it.sk - (it.first + j) * 128 - row0);  // of the warp's that exist
           const uint32_t my_scale = lane < rows ? staged_scale(code_scale[0], code_select[0], from, row0 + lane) : 127u;
           const uint32_t fits = __ballot_sync(0xffffffffu, my_scale >= 112 && my_scale <= 134);
           // Four lanes have the four chunks of 16 codes that make a row of a box, and the eight lanes of a shared-memory
@@ -731,7 +734,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           const int in8 = lane & 4 ? lane >> 3 ^ 5 : lane >> 3, quarter = lane & 3;
           const uint32_t ld = row0 * 128 + in8 * 128 + ((quarter ^ in8) << 4), st = row0 * 128 + in8 * 128 + ((quarter * 2 ^ in8) << 4);
 #pragma unroll 2
-          for (int k = 0; k < 4; ++k) {  // rows 8 k to 8 k + 7 of the warp's 32
+          for (int k = 0; k < T::kVRows / 8; ++k) {  // rows 8 k to 8 k + 7 of the warp's
             const uint32_t byte = __shfl_sync(0xffffffffu, my_scale, 8 * k + in8);
             const uint32_t h = (byte == 112 ? 0x0200u : (byte - 112) << 10) * 0x10001u;  // 2^(byte - 127) in fp16, twice
             const bool plain = (fits >> (k & 2) * 8 & 0xffffu) == 0xffffu;
@@ -764,11 +767,11 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           }
           // rows behind the entry's end: zeros, whatever the page holds there
           __syncwarp();
-          if (lane >= rows) {
+          if (lane >= rows && lane < T::kVRows) {
             for (int i = 0; i < 8 * T::kBoxes; ++i)
               sts128(to_smem + (i >> 3) * T::kBoxBytes + (row0 + lane) * 128 + (i & 7) * 16, 0, 0, 0, 0);
           }
-          if (lane < 2) v_bf16[slot][2 * (warp - 12) + lane] = (fits >> (16 * lane) & 0xffffu) != 0xffffu;
+          if (lane < T::kVRows / 16) v_bf16[slot][T::kVRows / 16 * (warp - 12) + lane] = (fits >> (16 * lane) & 0xffffu) != 0xffffu;
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
