@@ -499,24 +499,37 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           if (kBf16) c *= q_scale[piece & 3];
           c *= scale_value(k_scale[n & 3][tid]);
         }
+        // The exponentials' arguments: with 16 rows they stay in registers between the vote and the exponentials, with more
+        // they are formed twice.
+        float x[16];
+        auto arguments = [&](int r0) {
+          uint32_t s[16];
+          tmem_ld16(tS + r0, s);
+          tmem_wait_ld();
+          const uint64_t c2 = pack2f(c, c);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const float4 g = *reinterpret_cast<const float4*>(&row_neg[r0 + i]);
+            uint32_t a, b;
+            unpack2(fma2(pack2(s[i], s[i + 1]), c2, pack2f(g.x, g.y)), a, b);
+            x[i] = __uint_as_float(a), x[i + 1] = __uint_as_float(b);
+            unpack2(fma2(pack2(s[i + 2], s[i + 3]), c2, pack2f(g.z, g.w)), a, b);
+            x[i + 2] = __uint_as_float(a), x[i + 3] = __uint_as_float(b);
+          }
+        };
         if (j > 0) {
           // would an exponential be too large?  (2^10: P has to stay far from the 65504 of fp16)
           float top = -CUDART_INF_F;
 #pragma unroll
           for (int r0 = 0; r0 < kRows; r0 += 16) {
-            uint32_t s[16];
-            tmem_ld16(tS + r0, s);
-            tmem_wait_ld();
+            arguments(r0);
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const float4 g = *reinterpret_cast<const float4*>(&row_neg[r0 + i]);
-              top = max3_nan(top, fmaf(__uint_as_float(s[i]), c, g.x), fmaf(__uint_as_float(s[i + 1]), c, g.y));
-              top = max3_nan(top, fmaf(__uint_as_float(s[i + 2]), c, g.z), fmaf(__uint_as_float(s[i + 3]), c, g.w));
-            }
+            for (int i = 0; i < 16; i += 2) top = max3_nan(top, x[i], x[i + 1]);
           }
           force = vote_any(1, 128, force || (key < it.sk && !(top <= 10.f)));
         }
         const bool all_seen = key0 + 127 <= least;
+        const bool renewed = force;
         if (force) {
           // a new reference for every row: its largest score so far
 #pragma unroll 1
@@ -586,14 +599,10 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         const uint32_t dst = p_smem + b * T::kPBytes + p_key;
 #pragma unroll
         for (int r0 = 0; r0 < kRows; r0 += 16) {
-          uint32_t s[16];
-          tmem_ld16(tS + r0, s);
-          tmem_wait_ld();
+          if (kRows > 16 || renewed) arguments(r0);
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            const float4 g = *reinterpret_cast<const float4*>(&row_neg[r0 + i]);
-            float e[4] = {fast_exp2(fmaf(__uint_as_float(s[i]), c, g.x)), fast_exp2(fmaf(__uint_as_float(s[i + 1]), c, g.y)),
-                          fast_exp2(fmaf(__uint_as_float(s[i + 2]), c, g.z)), fast_exp2(fmaf(__uint_as_float(s[i + 3]), c, g.w))};
+            float e[4] = {fast_exp2(x[i]), fast_exp2(x[i + 1]), fast_exp2(x[i + 2]), fast_exp2(x[i + 3])};
             if (!all_seen) {
               const int4 last = *reinterpret_cast<const int4*>(&row_last[r0 + i]);
               e[0] = key <= last.x ? e[0] : 0.f;
