@@ -164,23 +164,28 @@ struct PagedPlan {
   size_t bytes() const { return part_bytes + lse_bytes + item_bytes; }
 };
 
-// Rows (new tokens times query heads of a cache head) of up to 16, 32 or 64 run the kernel of few rows, more the one of many.
+// Rows (new tokens times query heads of a cache head) of up to 16, 32, 48 or 64 run the kernel of few rows, more the one of
+// many.  us, on the GPU alone: 64 rows over 16384 keys, one entry of 8 heads, few 31.6 / many 34.4; 64 over 8192, 32 entries,
+// 160 / 197; 40 rows of 8-bit caches of 8192, 8 entries of 4 heads, by 48 / 64 / many 33.6 / 37.3 / 46.2.
+// The least share of a block: a tile, because a piece more costs less than a tile more on a block's way: with 1 / 2 / 4 / 8
+// tiles, one row group of 8 heads over 512 keys 9.9 / 10.6 / 12.2 / 15.5, over 4096 keys 12.2 / 12.2 / 13.1 / 15.7.  Two with many
+// rows, whose pieces leave 256 rows to be joined: 512 rows over 2048 keys, 8 heads, with 2 / 4 / 8 24.2 / 30.3 / 42.3.
 PagedPlan plan_paged(const FmhaPagedFwdParams* p, int sms) {
   PagedPlan plan = {};
   const int group = p->heads_q / p->heads_k;
   const long long rows = (long long)p->seqlen_q * group;
   if (rows <= 64) {
-    plan.kernel_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    plan.kernel_rows = (int)(rows + 15) / 16 * 16;
     plan.tokens_per_block = p->seqlen_q;
     plan.rows_per_tile = (int)rows;
     plan.tiles = 1;
-    plan.min_share = 2;
+    plan.min_share = 1;
   } else {
     plan.kernel_rows = 256;
     plan.tokens_per_block = 128 / group * 2;
     plan.rows_per_tile = 128 / group * group;
     plan.tiles = 2;
-    plan.min_share = 4;
+    plan.min_share = 2;
   }
   plan.blocks_per_entry = (p->seqlen_q + plan.tokens_per_block - 1) / plan.tokens_per_block;
   plan.blocks = sms;
@@ -392,6 +397,7 @@ int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspac
     constexpr int D = DR == 64 ? 64 : 128;
     if (plan.kernel_rows == 16) return launch_few<D, DR, kBf16, kE4m3, 16>(p, plan, workspace, dev, s);
     if (plan.kernel_rows == 32) return launch_few<D, DR, kBf16, kE4m3, 32>(p, plan, workspace, dev, s);
+    if (plan.kernel_rows == 48) return launch_few<D, DR, kBf16, kE4m3, 48>(p, plan, workspace, dev, s);
     if (plan.kernel_rows == 64) return launch_few<D, DR, kBf16, kE4m3, 64>(p, plan, workspace, dev, s);
     return launch_many<D, DR, kBf16, kE4m3>(p, plan, workspace, dev, s);
   })

@@ -33,6 +33,13 @@
 // The code is kept small: the roles share an instruction cache, and a miss waits in the same queues as HBM's data.
 // With 135 KB of code (everything unrolled, waits among it) warps waited for instructions most of the time, and 64 entries
 // of 2048 to 16384 keys in 8 bits took three times as long as their bytes.
+//
+// What bounds it.  16 bits, head dimension 128: HBM (32 entries of 2048 to 16384 keys, 32 query heads over 8: 182 us for 1.21
+// GB, 6.6 TB/s, the rate of a copy).  Otherwise a tile's way through the softmax warps: 1470 clk at head dimension 64, 16
+// bits, where 32 KB come in 1370 (16 entries of 16 heads: 4.3 TB/s), and 2200 to 2800 clk beside the converting warps, which
+// wait for it (64 entries in 8 bits: 309 us, 3.9 TB/s).  Short calls: 10 us of start, first loads, last tile and join.
+// A second group of softmax warps, which takes every other tile, was tried twice and taken back: 16 bits no faster, 8 bits
+// 309 -> 359 (four warps for V) and 393 (eight; 80 registers a thread), only head dimension 64 in 8 bits gained (296 -> 270).
 #pragma once
 #include <cuda.h>
 
@@ -49,10 +56,10 @@ struct FewTraits {
   static constexpr int kQBytes = kBoxes * kQBoxBytes;
   static constexpr int kPBytes = 2 * kRows * 128;
   // ring of K and V (16 bits), or of V alone and of codes (8 bits)
-  static constexpr int kStages = kE4m3 ? (D == 128 ? 3 : 4) : D == 128 ? (kRows == 16 ? 6 : 5) : (kRows == 64 ? 9 : 12);
-  static constexpr int kCodeStages = !kE4m3 ? 0 : D == 128 && kRows == 64 ? 4 : 6;
+  static constexpr int kStages = kE4m3 ? (D == 128 ? 3 : 4) : D == 128 ? (kRows == 16 ? 6 : 5) : (kRows >= 48 ? 9 : 12);
+  static constexpr int kCodeStages = !kE4m3 ? 0 : D == 128 && kRows >= 48 ? 4 : 6;
   static constexpr int kCodeBytes = 128 * 128;
-  static constexpr int kQBufs = D == 128 && (kRows == 64 || (kE4m3 && kRows == 32)) ? 1 : 2;
+  static constexpr int kQBufs = D == 128 && (kRows >= 48 || (kE4m3 && kRows == 32)) ? 1 : 2;
   static constexpr int kItemStages = 8;
   // warps that convert V: as many as the registers of the softmax's row sums leave room for
   static constexpr int kVWarps = kRows == 16 ? 8 : 4, kVRows = 128 / kVWarps;
@@ -60,7 +67,7 @@ struct FewTraits {
   static constexpr int kSmemBytes =
       1024 + kStages * kTileBytes + kCodeStages * kCodeBytes + kQBufs * kQBytes + 2 * kPBytes;
   static_assert(kSmemBytes <= 230400, "the rest of the 227 KB is for what is declared in the kernel");
-  static constexpr int kTmemCols = !kE4m3 ? 4 * kRows : kRows == 64 ? 512 : 256;
+  static constexpr int kTmemCols = !kE4m3 ? (kRows == 48 ? 256 : 4 * kRows) : kRows >= 48 ? 512 : 256;
   // 8-bit caches are multiplied in fp16 (see the converting warps)
   static constexpr uint32_t kIdescQK = umma_idesc_f16(128, kRows, 0, 0, kBf16 && !kE4m3);
   static constexpr uint32_t kIdescPV = umma_idesc_f16(128, kRows, 1, 0, kBf16 && !kE4m3);

@@ -251,6 +251,19 @@ def test_missing_pages_are_keys_of_zero():
 
 
 # ------------------------------------------------------------------------------------------ shapes and memory
+@pytest.mark.parametrize("n", [15, 16, 17, 32, 33, 47, 48, 49, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("d,dtype,e4m3", [(128, BF16, False), (64, F16, True), (96, BF16, True), (128, F16, True), (64, BF16, False)])
+def test_numbers_of_rows_at_the_kernels_ends(n, d, dtype, e4m3):
+    from flash_attn_v100 import flash_attn_paged_func
+
+    c = Cache([700, 260, 128], 2, d, 32, dtype, e4m3, seed=n)
+    q = _q(3, n, 2, d, dtype, n)
+    new = [n, n // 2, 1]
+    for causal in (True, False):
+        got = flash_attn_paged_func(q, *c.args(), c.seqused_k, _i32(new), causal=causal, return_lse=True, **c.scales())
+        check_attention(got, q, c, d ** -0.5, causal, new)
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("n", [1, 33])
 def test_many_entries_and_lengths_beyond_their_pages(e4m3, n):
