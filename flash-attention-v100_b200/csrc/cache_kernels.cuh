@@ -151,10 +151,13 @@ __device__ __forceinline__ void write_row(const PagedCache& c, int page, int slo
   }
 }
 
-// Rows that a thread of either kernel has: what bounds them is the chain of loads from an entry's length by its table to
-// the row's place, and more rows side by side hide it.  One row / four, us: four chunks of up to 4096 tokens into an 8-bit cache
-// WRITE_ONE / WRITE_FOUR, eight conversations of 1024 to 8192 tokens out of one READ_ONE / READ_FOUR.
-constexpr int kCacheRows = 4;
+// Rows that a thread has: what bounds both kernels is the chain of loads from an entry's length by its table to the row's
+// place, and then, in 8 bits, the conversion (ALU 47 and 63 % busy); more rows side by side hide the chain, more registers
+// leave room for fewer threads.  On the GPU alone, 1 / 2 / 4 rows, us: four chunks of up to 4096 tokens into an 8-bit cache (50 MB)
+// 18.5 / 17.3 / 17.7, three of 1000 in 16 bits (37 MB) 8.0 / 7.5 / 7.5; eight conversations of 1024 to 8192 tokens out of an
+// 8-bit cache (345 MB) 78.9 / 66.1 / 59.3 (5.8 TB/s, 89 % of a copy's rate), five of 252 to 2016 in 16 bits (65 MB) 11.7 / 12.1 /
+// 12.3.  (The magnitudes by their bits instead of as numbers: 22.5 -> 20.0 with the launch.)
+constexpr int kWriteRows = 2, kReadRows = 4;
 
 // New rows into their pages.  kLanes threads a row (8 elements each), K and V of the same row by the same threads, so
 // that the place is worked out once.
@@ -162,15 +165,15 @@ template <int DR, bool kBf16, bool kE4m3>
 __global__ void __launch_bounds__(256) cache_write_kernel(const CacheWriteArgs a) {
   constexpr int kLanes = DR == 64 ? 8 : 16;  // (96: four of sixteen idle)
   constexpr int kStep = 256 / kLanes;
-  const int r0 = (int)(blockIdx.x * (kStep * kCacheRows) + threadIdx.x / kLanes), sub = threadIdx.x % kLanes;
+  const int r0 = (int)(blockIdx.x * (kStep * kWriteRows) + threadIdx.x / kLanes), sub = threadIdx.x % kLanes;
   const bool in_row = sub * 8 < DR;
 #pragma unroll 1
   for (int z = blockIdx.y; z < a.batch; z += gridDim.y) {
     const int held = __ldg(a.seqlens + z), used = a.seqused == nullptr ? 0x7fffffff : __ldg(a.seqused + z);
-    uint4 x[kCacheRows][2];
-    int page[kCacheRows];
+    uint4 x[kWriteRows][2];
+    int page[kWriteRows];
 #pragma unroll
-    for (int k = 0; k < kCacheRows; ++k) {
+    for (int k = 0; k < kWriteRows; ++k) {
       const int r = r0 + k * kStep, i = (int)((unsigned)r / (unsigned)a.heads), h = r - i * a.heads;
       const long long t = (long long)held + i;
       x[k][0] = x[k][1] = make_uint4(0, 0, 0, 0);
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CacheWriteArgs a
       }
     }
 #pragma unroll
-    for (int k = 0; k < kCacheRows; ++k) {
+    for (int k = 0; k < kWriteRows; ++k) {
       if ((unsigned)page[k] >= (unsigned)a.cache.num_pages) continue;  // (the threads of a row share a shuffle, and skip it together)
       const int r = r0 + k * kStep, i = (int)((unsigned)r / (unsigned)a.heads), h = r - i * a.heads;
       write_row<DR, kBf16, kE4m3, kLanes>(a.cache, page[k], cache_page_row(a.cache, held + i), h, sub, in_row, x[k]);
@@ -207,21 +210,21 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) 
   constexpr unsigned kLanes = DR / 8, kBlockRows = 256 / kLanes;  // (96: 4 of 256 threads idle)
   const int in_block = (int)(threadIdx.x / kLanes), sub = (int)(threadIdx.x % kLanes);
   if (in_block >= (int)kBlockRows) return;
-  const int r0 = (int)(blockIdx.x * (kBlockRows * kCacheRows)) + in_block;
+  const int r0 = (int)(blockIdx.x * (kBlockRows * kReadRows)) + in_block;
 #pragma unroll 1
   for (int z = blockIdx.y; z < a.batch; z += gridDim.y) {
     const int sk = min(__ldg(a.seqused_k + z), cache_capacity(a.cache));
-    int page[kCacheRows];
+    int page[kReadRows];
 #pragma unroll
-    for (int k = 0; k < kCacheRows; ++k) {
+    for (int k = 0; k < kReadRows; ++k) {
       const int r = r0 + k * (int)kBlockRows, t = (int)((unsigned)r / (unsigned)a.heads);
       page[k] = -1;
       if (r < a.rows && t < sk) page[k] = cache_entry(a.cache, z, t);
     }
-    uint4 x[kCacheRows][2] = {};
-    uint32_t scale[kCacheRows][2] = {};
+    uint4 x[kReadRows][2] = {};
+    uint32_t scale[kReadRows][2] = {};
 #pragma unroll
-    for (int k = 0; k < kCacheRows; ++k) {
+    for (int k = 0; k < kReadRows; ++k) {
       if ((unsigned)page[k] >= (unsigned)a.cache.num_pages) continue;
       const int r = r0 + k * (int)kBlockRows, t = (int)((unsigned)r / (unsigned)a.heads), h = r - t * a.heads;
       const int slot = cache_page_row(a.cache, t);
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) 
       }
     }
 #pragma unroll
-    for (int k = 0; k < kCacheRows; ++k) {
+    for (int k = 0; k < kReadRows; ++k) {
       const int r = r0 + k * (int)kBlockRows, t = (int)((unsigned)r / (unsigned)a.heads), h = r - t * a.heads;
       if (r >= a.rows) break;
       if constexpr (kE4m3) {

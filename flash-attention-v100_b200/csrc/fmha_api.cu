@@ -950,7 +950,7 @@ const char* fmha_status_string(int status) {
     case FMHA_ERR_BAD_SHAPE: return "sizes must be positive and scale finite and non-zero";
     case FMHA_ERR_BAD_STRIDE: return "strides must be positive multiples of 8 elements";
     case FMHA_ERR_BAD_ALIGNMENT: return "pointers must be 16-byte aligned";
-    case FMHA_ERR_WORKSPACE: return "backward workspace missing or too small";
+    case FMHA_ERR_WORKSPACE: return "workspace missing or too small";
     case FMHA_ERR_TENSOR_MAP: return "cuTensorMapEncodeTiled rejected a tensor";
     case FMHA_ERR_NO_DEVICE: return "CUDA driver entry point unavailable";
     case FMHA_ERR_LAUNCH: return "kernel launch failed";
@@ -960,7 +960,7 @@ const char* fmha_status_string(int status) {
   }
 }
 
-const char* fmha_version(void) { return "0.3.0"; }
+const char* fmha_version(void) { return "0.4.0"; }
 
 #ifdef FMHA_TIMELINE
 // debug builds only: device buffer (>= 3 * 512 int64) and the CTA whose events are recorded

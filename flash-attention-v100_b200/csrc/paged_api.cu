@@ -328,7 +328,7 @@ int fmha_cache_write(const FmhaCacheWriteParams* p, void* stream) {
   a.heads = p->heads;
   a.batch = p->batch;
   a.rows = (int)rows;
-  const dim3 grid = cache_grid(a.rows, fmha::kCacheRows * (256 / (p->head_dim == 64 ? 8 : 16)), p->batch);
+  const dim3 grid = cache_grid(a.rows, fmha::kWriteRows * (256 / (p->head_dim == 64 ? 8 : 16)), p->batch);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format,
                       fmha::cache_write_kernel<DR, kBf16, kE4m3><<<grid, 256, 0, s>>>(a);)
@@ -358,7 +358,7 @@ int fmha_cache_read(const FmhaCacheReadParams* p, void* stream) {
   a.heads = p->heads;
   a.batch = p->batch;
   a.rows = (int)rows;
-  const dim3 grid = cache_grid(a.rows, fmha::kCacheRows * (256 / (p->head_dim / 8)), p->batch);
+  const dim3 grid = cache_grid(a.rows, fmha::kReadRows * (256 / (p->head_dim / 8)), p->batch);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   FMHA_DISPATCH_CACHE(p->head_dim, p->dtype, p->cache.format,
                       fmha::cache_read_kernel<DR, kBf16, kE4m3><<<grid, 256, 0, s>>>(a);)
