@@ -37,13 +37,9 @@ __device__ __forceinline__ int cache_page_row(const PagedCache& c, int t) {
 // tokens an entry can hold at most (fits: checked on the host)
 __device__ __forceinline__ int cache_capacity(const PagedCache& c) { return c.max_pages * c.page_size; }
 
-// what the table has for token `t` of entry z; its page, -1 where the table names none
+// what the table has for token `t` of entry z: a page, where it is less than num_pages (as an unsigned number)
 __device__ __forceinline__ int cache_entry(const PagedCache& c, int z, int t) {
   return __ldg(c.table + z * c.table_stride + cache_page_index(c, t));
-}
-__device__ __forceinline__ int cache_page(const PagedCache& c, int z, int t) {
-  const int page = cache_entry(c, z, t);
-  return (unsigned)page < (unsigned)c.num_pages ? page : -1;
 }
 
 // 2^(byte - 127), the value of a scale byte (255 is NaN; 0 is 2^-127, a subnormal)

@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       while (ok) {
         const PagedPiece it = take_item();
         if (it.id < 0) break;
-  #pragma unroll 1
+#pragma unroll 1
         for (int j = 0; j < it.tiles; ++j, ++n) {
           const uint32_t b = n & 1, at = 2 * n, slot = at % T::kCodeStages;
           ok = rolled_wait_warp(smem_u32(&bar_code_full[slot]), at / T::kCodeStages & 1, &abort_word, 20);
@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           tc_fence_after();
           const uint32_t src = code_smem + slot * T::kCodeBytes + tid * 128;
           k_scale[n & 3][tid] = (uint8_t)staged_scale(code_scale[0], code_select[0], slot, tid);
-  #pragma unroll 2
+#pragma unroll 2
           for (int i = 0; i < T::kChunks; i += 2) {  // 32 elements, 16 columns of tensor memory
             uint32_t w[16];
 #pragma unroll
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       while (ok) {
         const PagedPiece it = take_item();
         if (it.id < 0) break;
-  #pragma unroll 1
+#pragma unroll 1
         for (int j = 0; j < it.tiles; ++j, ++n) {
           const uint32_t slot = n % kStages, at = 2 * n + 1, from = at % T::kCodeStages;
           ok = rolled_wait_warp(smem_u32(&bar_code_full[from]), at / T::kCodeStages & 1, &abort_word, 22) &&

@@ -53,7 +53,6 @@ struct ManyTraits {
   static_assert(kRegsOther <= kRegsLaunch && kRegsSoftmax >= kRegsLaunch &&
                     2 * kRegsSoftmax + (kThreads / 128 - 2) * kRegsOther <= kThreads / 128 * kRegsLaunch,
                 "setmaxnreg.dec must not raise, .inc must not lower the launch's registers, nor ask for more than it has");
-  static constexpr int kChunks = DR / 16;
 };
 
 template <int D, int DR, bool kBf16, bool kE4m3>
