@@ -649,7 +649,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       named_bar_sync(1, 128);
       if (tid < kRows) {
         const float sum = (warp_part[0][tid] + warp_part[1][tid]) + (warp_part[2][tid] + warp_part[3][tid]);
-        row_scale[tid] = sum == 0.f ? 0.f : 1.f / sum;
+        // (a score of infinity: inf / inf is NaN, and 1 / inf would be the 0 of a row without a key)
+        row_scale[tid] = sum == 0.f ? 0.f : isinf(sum) ? CUDART_NAN_F : 1.f / sum;
         if (row_here) *my_lse = sum == 0.f ? -CUDART_INF_F : (ref + log2f(sum)) * 0.6931471805599453f;
       }
       named_bar_sync(1, 128);

@@ -235,6 +235,52 @@ def test_not_finite_stays_in_its_rows(n, e4m3):
     assert torch.equal(o[0, seen, :4], o0[0, seen, :4])
 
 
+@pytest.mark.parametrize("n", [1, 6, 80])
+@pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (BF16, True), (F16, False), (F16, True)])
+def test_an_infinite_score_is_no_answer(n, dtype, e4m3):
+    """An infinite element of a query makes scores of infinity, and inf / inf is NaN: in the whole row, and in no other."""
+    from flash_attn_v100 import flash_attn_paged_func
+
+    c = Cache([700, 90], 2, 64, 32, dtype, e4m3, seed=11)
+    clean = _q(2, n, 8, 64, dtype, 12)
+    call = lambda q: flash_attn_paged_func(q, *c.args(), c.seqused_k, causal=True, return_lse=True, **c.scales())  # noqa: E731
+    o0, l0 = call(clean)
+    q = clean.clone()
+    rows = [(0, n - 1, 1), (0, n // 2, 6), (1, n - 1, 0)]
+    for i, (z, t, h) in enumerate(rows):
+        q[z, t, h, 9 + i] = math.inf if i % 2 else -math.inf
+    o, lse = call(q)
+    for z, t, h in rows:
+        assert torch.isnan(o[z, t, h]).all() and not torch.isfinite(lse[z, h, t]) and lse[z, h, t] != -math.inf
+        o[z, t, h], lse[z, h, t] = o0[z, t, h], l0[z, h, t]
+    check_attention((o, lse), clean, c, 0.125, True)
+
+
+@pytest.mark.parametrize("n", [1, 6, 80])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scores_of_minus_infinity_have_no_weight(n, dtype):
+    """Keys of -inf in one element (16 bits): to queries that are positive there they are as good as absent, over whole tiles
+    too; queries that are negative there have no answer."""
+    from flash_attn_v100 import flash_attn_paged_func
+
+    gone = 150
+    c = Cache([700], 2, 64, 32, dtype, False, seed=13)
+    page, slot = c.where(0, range(gone))
+    c.k_cache[page, slot, :, 5] = -math.inf
+    q = _q(1, n, 8, 64, dtype, 14)
+    q[..., 5] = q[..., 5].abs() + 0.125
+    clean, bad = q.clone(), [(n - 1, 2), (n // 2, 7)]
+    for t, h in bad:
+        q[0, t, h, 5] *= -1
+    o0, l0 = flash_attn_paged_func(clean, *c.args(), c.seqused_k, causal=True, return_lse=True)
+    o, lse = flash_attn_paged_func(q, *c.args(), c.seqused_k, causal=True, return_lse=True)
+    for t, h in bad:
+        assert torch.isnan(o[0, t, h]).all() and not torch.isfinite(lse[0, h, t]) and lse[0, h, t] != -math.inf
+        o[0, t, h], lse[0, h, t] = o0[0, t, h], l0[0, h, t]
+    c.k, c.v, c.lens = [c.k[0][gone:]], [c.v[0][gone:]], [c.lens[0] - gone]
+    check_attention((o, lse), clean, c, 0.125, True)
+
+
 def test_missing_pages_are_keys_of_zero():
     from flash_attn_v100 import flash_attn_paged_func, paged_cache_read
 
