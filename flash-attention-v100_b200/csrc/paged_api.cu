@@ -151,6 +151,22 @@ int make_rows_map(CUtensorMap* map, const void* base, int Z, int N, int H, int D
   return r == CUDA_SUCCESS ? FMHA_OK : FMHA_ERR_TENSOR_MAP;
 }
 
+// sizes of an attention call, which the size query and the call itself have to agree on
+int check_paged_sizes(const FmhaPagedFwdParams* p) {
+  if (const int rc = check_sizes(p->batch, p->heads_k, p->head_dim, p->dtype)) return rc;
+  if (p->heads_q <= 0 || p->heads_q % p->heads_k != 0 || p->heads_q / p->heads_k > 128 || p->seqlen_q < 0)
+    return FMHA_ERR_BAD_SHAPE;
+  return FMHA_OK;
+}
+// items are counted in 32 bits, and so are the blocks that join them (eight rows each)
+int check_paged_limits(const FmhaPagedFwdParams* p) {
+  if ((long long)p->seqlen_q * p->heads_q >= (1ll << 31) ||
+      (double)p->batch * p->heads_q * (p->seqlen_q / 128 + 2.0) >= 2147483648.0 ||
+      (double)p->batch * p->heads_q * (p->seqlen_q + 256.0) >= 8 * 2147483648.0)
+    return FMHA_ERR_TOO_LARGE;
+  return FMHA_OK;
+}
+
 // How a call is cut (paged_work.cuh) and what that takes.
 struct PagedPlan {
   int kernel_rows;       // rows of an item that the kernel has room for
@@ -187,7 +203,7 @@ PagedPlan plan_paged(const FmhaPagedFwdParams* p, int sms) {
     plan.tiles = 2;
     plan.min_share = 2;
   }
-  plan.blocks_per_entry = (p->seqlen_q + plan.tokens_per_block - 1) / plan.tokens_per_block;
+  plan.blocks_per_entry = (int)(((long long)p->seqlen_q + plan.tokens_per_block - 1) / plan.tokens_per_block);
   plan.blocks = sms;
   const size_t items = (size_t)p->batch * plan.blocks_per_entry * p->heads_k;
   plan.part_bytes = (size_t)2 * plan.blocks * plan.kernel_rows * p->head_dim * sizeof(float);
@@ -366,22 +382,20 @@ int fmha_cache_read(const FmhaCacheReadParams* p, void* stream) {
 }
 
 size_t fmha_paged_fwd_workspace_bytes(const FmhaPagedFwdParams* p) {
-  if (p == nullptr || p->batch <= 0 || p->heads_k <= 0 || p->heads_q < p->heads_k || p->seqlen_q <= 0 || p->head_dim <= 0)
+  if (p == nullptr || check_paged_sizes(p) != FMHA_OK || p->batch == 0 || p->seqlen_q == 0 ||
+      check_paged_limits(p) != FMHA_OK)
     return 0;
   return plan_paged(p, sm_count(current_device())).bytes();
 }
 
 int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspace_bytes, void* stream) {
   if (p == nullptr) return FMHA_ERR_NULL_POINTER;
-  int rc = check_sizes(p->batch, p->heads_k, p->head_dim, p->dtype);
+  int rc = check_paged_sizes(p);
   if (rc) return rc;
-  if (p->heads_q <= 0 || p->heads_q % p->heads_k != 0 || p->heads_q / p->heads_k > 128 || p->seqlen_q < 0 ||
-      !std::isfinite(p->scale) || p->scale == 0.f)
-    return FMHA_ERR_BAD_SHAPE;
+  if (!std::isfinite(p->scale) || p->scale == 0.f) return FMHA_ERR_BAD_SHAPE;
   if (p->batch == 0 || p->seqlen_q == 0) return FMHA_OK;
   if ((rc = check_cache(p->cache, p->heads_k))) return rc;
-  if ((long long)p->seqlen_q * p->heads_q >= (1ll << 31) ||
-      (long long)p->batch * p->heads_q * (p->seqlen_q / 128 + 2ll) >= (1ll << 31)) return FMHA_ERR_TOO_LARGE;
+  if ((rc = check_paged_limits(p))) return rc;
   if (p->q == nullptr || p->o == nullptr || p->lse == nullptr || p->seqused_k == nullptr) return FMHA_ERR_NULL_POINTER;
   if (!aligned16(p->q) || !aligned16(p->o) || !aligned16(workspace)) return FMHA_ERR_BAD_ALIGNMENT;
   if ((rc = check_strides(p->q_strides, p->seqlen_q, p->heads_q, p->batch))) return rc;
