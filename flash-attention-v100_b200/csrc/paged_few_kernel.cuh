@@ -321,8 +321,10 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       if (round > 0 && !rolled_wait_warp(smem_u32(&bar_q_free[b]), (round - 1) & 1, &abort_word, 24)) break;
       if constexpr (kE4m3 && kBf16) {
         // Q in fp16, like K: divided by the power of two that brings its largest value to [2^14, 2^15).  What is less
-        // than 2^-28 of that value loses bits, nothing is off by more than 2^-39 of it.
+        // than 2^-28 of that value loses bits, nothing is off by more than 2^-39 of it.  Rows behind the entry's new tokens may
+        // hold anything: they have no say in it, and become zeros.
         const int total = p.seqlen_q * p.group * (DR / 8);  // chunks of 8 elements
+        const int real = min(p.seqlen_q, it.sq - it.token0) * p.group * (DR / 8);
         const uint16_t* src = p.q + it.z * p.q_batch + it.token0 * p.q_row + it.h * p.group * p.q_head;
         auto chunk_of = [&](int n) {
           const int r = n / (DR / 8), t = row_token(p, r);
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         };
         uint32_t top = 0;  // exponent fields of finite values
 #pragma unroll 1
-        for (int n = lane; n < total; n += 32) {
+        for (int n = lane; n < real; n += 32) {
           const uint4 x = chunk_of(n);
           for (uint32_t w : {x.x, x.y, x.z, x.w})
             for (uint32_t ex : {w >> 7 & 0xffu, w >> 23 & 0xffu}) top = ex == 255 ? top : max(top, ex);
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
 #pragma unroll 1
         for (int n = lane; n < total; n += 32) {
           float f[8];
-          unpack8<__nv_bfloat16>(chunk_of(n), f);
+          unpack8<__nv_bfloat16>(n < real ? chunk_of(n) : make_uint4(0, 0, 0, 0), f);
           const int r = n / (DR / 8), c = n % (DR / 8);
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] = f[i] * s0 * s1;
