@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   __shared__ uint64_t bar_q_full[2], bar_q_free[2], bar_s_full[2], bar_s_free[2], bar_p_full[2], bar_p_free[2],
       bar_o_full[2], bar_o_free[2];
   __shared__ float warp_part[4][kRows];   // per warp: a row's maximum, or its sum
-  __shared__ __align__(16) float row_neg[kRows];    // minus the reference, 0 where there is no finite one
+  __shared__ __align__(16) float row_neg[kRows];    // minus the reference, 0 where there is no finite one, -inf for rows that see no key
   __shared__ __align__(16) float row_scale[kRows];  // what O is multiplied by
   __shared__ __align__(16) int row_last[kRows];     // last key a row sees
   __shared__ long long row_out[kRows];              // where a row of O lies, from its block's first row on
@@ -527,13 +527,15 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           }
         };
         if (j > 0) {
-          // would an exponential be too large?  (2^10: P has to stay far from the 65504 of fp16)
+          // Would an exponential be too large?  (2^10: P has to stay far from the 65504 of fp16.)  Rows that see no key, padding
+          // among them, have no say: their arguments are -inf, or NaN, which the maximum passes over.  (A NaN of a row that
+          // does see the key makes P and the row sum NaN whatever the reference is.)
           float top = -CUDART_INF_F;
 #pragma unroll
           for (int r0 = 0; r0 < kRows; r0 += 16) {
             arguments(r0);
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) top = max3_nan(top, x[i], x[i + 1]);
+            for (int i = 0; i < 16; i += 2) top = max3(top, x[i], x[i + 1]);
           }
           force = vote_any(1, 128, force || (key < it.sk && !(top <= 10.f)));
         }
@@ -561,7 +563,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             const float m = fmaxf(fmaxf(fmaxf(warp_part[0][tid], warp_part[1][tid]),
                                         fmaxf(warp_part[2][tid], warp_part[3][tid])), ref);
             row_scale[tid] = isinf(m) || isinf(ref) ? 1.f : fast_exp2(ref - m);
-            row_neg[tid] = isinf(m) ? 0.f : -m;
+            row_neg[tid] = row_last[tid] < 0 ? -CUDART_INF_F : isinf(m) ? 0.f : -m;
             ref = m;
             unset = m == -CUDART_INF_F && row_last[tid] > key0 + 127;
           }
