@@ -8,7 +8,8 @@
 // few dozen instructions, and what belongs to a key (is it visible) is worked out once per thread.  Row sums stay
 // partial per thread until the item ends.  The reference of a row's exponentials is its maximum over the first tile; a
 // later tile replaces it only where an exponential would exceed 2^10, so that an ordinary tile needs no maximum
-// across threads, only a vote.
+// across threads, only a vote.  P in fp16 is 2^5 times the exponential, 2^15 at most: its least step, 2^-24, is then 2^-29 of
+// the reference's weight, and a long tail of small weights is not lost.  The row sum has the factor, too.
 //
 //   warps 0-3   softmax: thread = key; P^T to shared memory; O^T (thread = element of the head) at the end
 //   warps 4, 7  MMA issuers, of S^T and of O^T
@@ -75,6 +76,8 @@ struct FewTraits {
   // V^T has D rows; with D = 64 the upper 64 of the 128 repeat the lower ones, unused
   static constexpr uint32_t kLboV = D == 128 ? kBoxBytes : 0;
   static constexpr int kChunks = DR / 16;  // 16-byte chunks of a row of codes
+  // P is 2^kLift times the exponential over the reference
+  static constexpr float kLift = kBf16 && !kE4m3 ? 0.f : 5.f;
 };
 
 __device__ __forceinline__ bool vote_any(uint32_t id, uint32_t count, bool mine) {
@@ -134,7 +137,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   __shared__ uint64_t bar_q_full[2], bar_q_free[2], bar_s_full[2], bar_s_free[2], bar_p_full[2], bar_p_free[2],
       bar_o_full[2], bar_o_free[2];
   __shared__ float warp_part[4][kRows];   // per warp: a row's maximum, or its sum
-  __shared__ __align__(16) float row_neg[kRows];    // minus the reference, 0 where there is no finite one, -inf for rows that see no key
+  // kLift minus the reference, 0 where there is no finite one, -inf for rows that see no key
+  __shared__ __align__(16) float row_neg[kRows];
   __shared__ __align__(16) float row_scale[kRows];  // what O is multiplied by
   __shared__ __align__(16) int row_last[kRows];     // last key a row sees
   __shared__ long long row_out[kRows];              // where a row of O lies, from its block's first row on
@@ -527,7 +531,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           }
         };
         if (j > 0) {
-          // Would an exponential be too large?  (2^10: P has to stay far from the 65504 of fp16.)  Rows that see no key, padding
+          // Would an exponential be too large?  (2^10 over the reference: P has to stay below the 65504 of fp16.)  Rows that see no key, padding
           // among them, have no say: their arguments are -inf, or NaN, which the maximum passes over.  (A NaN of a row that
           // does see the key makes P and the row sum NaN whatever the reference is.)
           float top = -CUDART_INF_F;
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
 #pragma unroll
             for (int i = 0; i < 16; i += 2) top = max3(top, x[i], x[i + 1]);
           }
-          force = vote_any(1, 128, force || (key < it.sk && !(top <= 10.f)));
+          force = vote_any(1, 128, force || (key < it.sk && !(top <= 10.f + T::kLift)));
         }
         const bool all_seen = key0 + 127 <= least;
         const bool renewed = force;
@@ -563,7 +567,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             const float m = fmaxf(fmaxf(fmaxf(warp_part[0][tid], warp_part[1][tid]),
                                         fmaxf(warp_part[2][tid], warp_part[3][tid])), ref);
             row_scale[tid] = isinf(m) || isinf(ref) ? 1.f : fast_exp2(ref - m);
-            row_neg[tid] = row_last[tid] < 0 ? -CUDART_INF_F : isinf(m) ? 0.f : -m;
+            row_neg[tid] = row_last[tid] < 0 ? -CUDART_INF_F : isinf(m) ? 0.f : T::kLift - m;
             ref = m;
             unset = m == -CUDART_INF_F && row_last[tid] > key0 + 127;
           }
@@ -652,10 +656,11 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       }
       named_bar_sync(1, 128);
       if (tid < kRows) {
+        constexpr float kUnlift = T::kLift == 0.f ? 1.f : 1.f / 32.f;
         const float sum = (warp_part[0][tid] + warp_part[1][tid]) + (warp_part[2][tid] + warp_part[3][tid]);
         // (a score of infinity: inf / inf is NaN, and 1 / inf would be the 0 of a row without a key)
         row_scale[tid] = sum == 0.f ? 0.f : isinf(sum) ? CUDART_NAN_F : 1.f / sum;
-        if (row_here) *my_lse = sum == 0.f ? -CUDART_INF_F : (ref + log2f(sum)) * 0.6931471805599453f;
+        if (row_here) *my_lse = sum == 0.f ? -CUDART_INF_F : (ref + log2f(sum * kUnlift)) * 0.6931471805599453f;
       }
       named_bar_sync(1, 128);
       const uint32_t ob = piece & 1;

@@ -1,0 +1,55 @@
+"""GPU tests of the paged attention's numbers: weights that are small but many, scores and factors at the ends of fp32."""
+import pytest
+import torch
+
+from tests.paged_helpers import UNIT, Cache, attend64
+from tests.test_gpu_paged_use import Held
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _q(z, n, h, d, dtype, seed=1, size=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn((z, n, h, d), generator=g) * size).to(dtype).cuda()
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _attend(q, c, lens, new=None, causal=True, **kw):
+    from flash_attn_v100 import flash_attn_paged_func
+
+    return flash_attn_paged_func(q, *c.args(), lens, None if new is None else _i32(new), causal=causal, return_lse=True,
+                                 **c.scales(), **kw)
+
+
+@pytest.mark.parametrize("n", [1, 16, 17, 33, 49, 64])
+@pytest.mark.parametrize("dtype,e4m3", [(BF16, True), (F16, True), (F16, False), (BF16, False)])
+def test_small_shares_add_up(n, dtype, e4m3):
+    """A first key that has all the weight but 2^-26 for each of 8191 others, and a value of zero: the output is what the
+    others leave, 1.2e-4.  P of up to 64 rows is 2^5 times the exponential over the reference, so an fp16 P, whose least step
+    is 2^-24, is off by 2^-30 of the first key's at most, an output by 2^-30 of the sum of |v| over the keys seen."""
+    from flash_attn_v100 import paged_cache_read, paged_cache_write
+
+    z, h, d, length = 10, 16, 64, 8192  # (more items than SMs: few of them are cut)
+    c = Cache([0] * z, h, d, 64, dtype, e4m3, room=length)
+    k, v = (torch.zeros((z, length, h, d), dtype=dtype, device="cuda") for _ in range(2))
+    k[:, 0, :, 0] = 72.0
+    v[:, 1:] = 1.0 + torch.arange(8, device="cuda", dtype=dtype).repeat(8) / 8
+    paged_cache_write(k, v, *c.args(), _i32([0] * z), **c.scales())
+    lens = [length] * z
+    held = Held(*paged_cache_read(*c.args(), _i32(lens), length, dtype=dtype, **c.scales()), lens, e4m3)
+    q = torch.zeros((z, n, h, d), dtype=dtype, device="cuda")
+    q[..., 0] = 2.0
+    o, lse = _attend(q, c, _i32(lens), causal=False)
+    r_o, r_lse, a, b, size = attend64(q[:2], held, 0.125, False)
+    e = 2.0 ** -23 * ((d + 4) * float(size.max()) + 8)
+    u = UNIT[dtype]
+    limit = u * (1 + u) * (a + r_o.abs()) + 4 * e * a + 2.0 ** -24
+    if dtype == F16 or e4m3:
+        limit = limit + 2.0 ** -30 * b
+    assert ((o[:2].double() - r_o).abs() <= limit).all()
+    assert ((lse[:2].double() - r_lse).abs() <= e + 2.0 ** -22 * r_lse.abs()).all()
