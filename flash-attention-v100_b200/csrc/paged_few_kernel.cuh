@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       float l[kRows];
 #pragma unroll
       for (int r = 0; r < kRows; ++r) l[r] = 0.f;
-      bool force = true;  // some row has no reference yet
+      bool force = true;  // some row has no reference yet, or a very large one
 #pragma unroll 1
       for (int j = 0; j < it.tiles; ++j, ++n) {
         const uint32_t b = n & 1;
@@ -546,7 +546,9 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         const bool all_seen = key0 + 127 <= least;
         const bool renewed = force;
         if (force) {
-          // a new reference for every row: its largest score so far
+          // A new reference for every row: its largest score so far.  It is a rounded product, so this tile's scores become
+          // rounded products, too, before it is taken off: in one step, a score of 2^28 could come out at 2^4 over itself, or
+          // under.  Where a reference exceeds 2^20, every tile takes new ones.
 #pragma unroll 1
           for (int r0 = 0; r0 < kRows; r0 += 16) {
             uint32_t s[16];
@@ -556,20 +558,25 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             if (r0 == 0 && j == 0) named_bar_sync(1, 128);  // row_last is there
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float m = warp_max(key <= row_last[r0 + i] ? __uint_as_float(s[i]) * c : -CUDART_INF_F);
+              const float product = __uint_as_float(s[i]) * c;
+              s[i] = __float_as_uint(product);
+              const float m = warp_max(key <= row_last[r0 + i] ? product : -CUDART_INF_F);
               mine = lane == i ? m : mine;
             }
+            tmem_st16(tS + r0, s);
             if (lane < 16) warp_part[warp][r0 + lane] = mine;
           }
+          tmem_wait_st();
+          c = 1.f;
           named_bar_sync(1, 128);
-          bool unset = false;
+          bool unset = false;  // the next tile has to take references again
           if (tid < kRows) {
             const float m = fmaxf(fmaxf(fmaxf(warp_part[0][tid], warp_part[1][tid]),
                                         fmaxf(warp_part[2][tid], warp_part[3][tid])), ref);
             row_scale[tid] = isinf(m) || isinf(ref) ? 1.f : fast_exp2(ref - m);
             row_neg[tid] = row_last[tid] < 0 ? -CUDART_INF_F : isinf(m) ? 0.f : T::kLift - m;
             ref = m;
-            unset = m == -CUDART_INF_F && row_last[tid] > key0 + 127;
+            unset = m == -CUDART_INF_F ? row_last[tid] > key0 + 127 : fabsf(m) > 1048576.f;
           }
           force = vote_any(1, 128, unset);
           if (j > 0) {

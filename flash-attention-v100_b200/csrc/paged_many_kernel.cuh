@@ -464,6 +464,11 @@ __global__ void __launch_bounds__(ManyTraits<D, DR, kBf16, kE4m3>::kThreads, 1)
     uint32_t phase_s = 0, phase_o = 0;  // parities of the next s_full[t], o_full[t]
     bool stored = false;  // a TMA store of this group may still be reading the staging box
 
+    // The reference is a rounded product.  Taken off in one step (fma), a key's own product is not rounded, and a score of 2^28
+    // could come out at 2^4 over itself, or under.  So beyond 2^20 the reference is NaN to the ordinary way, which then sends
+    // every round the other way, where a warp that has such a row rounds products first.  (Rounding them always: 3 % of a call.)
+    auto one_step = [](float neg) { return fabsf(neg) > 1048576.f ? CUDART_NAN_F : neg; };
+
     // The epilogue of a piece is done after the first round of the next one (see fwd_kernel.cuh).
     bool pending = false;
     float done_m = 0.f, done_l = 0.f;
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(ManyTraits<D, DR, kBf16, kE4m3>::kThreads, 1)
         lim -= it.first * 128;
       }
       float m_ref = -CUDART_INF_F;  // reference score of the running softmax (raw, unscaled)
-      float neg_mc = 0.f;           // -m_ref * c, 0 while there is no reference
+      float neg_mc = 0.f;           // -m_ref * c, 0 while there is no reference, NaN where that is too large for one step
       float l = 0.f;                // running sum of exp2((s - m_ref) * c)
 
       for (int j = 0; j < n || j == 0; ++j, lim -= 128) {
@@ -561,7 +566,22 @@ __global__ void __launch_bounds__(ManyTraits<D, DR, kBf16, kE4m3>::kThreads, 1)
                 }
               }
               m_ref = m_new;
-              neg_mc = isinf(m_ref) ? 0.f : -m_ref * c;
+              const float neg = isinf(m_ref) ? 0.f : -m_ref * c;
+              neg_mc = one_step(neg);
+              float factor = c;
+              if (__any_sync(0xffffffffu, isnan(neg_mc))) {
+                factor = 1.f;
+#pragma unroll 1
+                for (int ch = 0; ch < 4; ++ch) {
+                  uint32_t x[16];
+                  tmem_ld16(tS + half * 64 + ch * 16, x);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * c);
+                  tmem_st16(tS + half * 64 + ch * 16, x);
+                }
+                tmem_wait_st();
+              }
               sum = 0.f;
 #pragma unroll 1
               for (int ch = 0; ch < 2; ++ch) {
@@ -571,8 +591,8 @@ __global__ void __launch_bounds__(ManyTraits<D, DR, kBf16, kE4m3>::kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
                   const int col = half * 64 + ch * 32 + i;
-                  const float e0 = col <= lim ? fast_exp2(fmaf(__uint_as_float(x[i]), c, neg_mc)) : 0.f;
-                  const float e1 = col + 1 <= lim ? fast_exp2(fmaf(__uint_as_float(x[i + 1]), c, neg_mc)) : 0.f;
+                  const float e0 = col <= lim ? fast_exp2(fmaf(__uint_as_float(x[i]), factor, neg)) : 0.f;
+                  const float e1 = col + 1 <= lim ? fast_exp2(fmaf(__uint_as_float(x[i + 1]), factor, neg)) : 0.f;
                   sum += e0 + e1;
                   h[i >> 1] = pack16x2<kBf16>(e0, e1);
                 }
@@ -596,7 +616,7 @@ __global__ void __launch_bounds__(ManyTraits<D, DR, kBf16, kE4m3>::kThreads, 1)
                 mx[cc] = max3(mx[cc], __uint_as_float(s[cc][i]), __uint_as_float(s[cc][i + 1]));
             }
             m_ref = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-            neg_mc = isinf(m_ref) ? 0.f : -m_ref * c;
+            neg_mc = one_step(isinf(m_ref) ? 0.f : -m_ref * c);
           }
           half_round(std::integral_constant<int, 0>{});
           half_round(std::integral_constant<int, 1>{});

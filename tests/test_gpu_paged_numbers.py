@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.paged_helpers import UNIT, Cache, attend64
+from tests.paged_helpers import UNIT, Cache, attend64, check_attention
 from tests.test_gpu_paged_use import Held
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +53,32 @@ def test_small_shares_add_up(n, dtype, e4m3):
         limit = limit + 2.0 ** -30 * b
     assert ((o[:2].double() - r_o).abs() <= limit).all()
     assert ((lse[:2].double() - r_lse).abs() <= e + 2.0 ** -22 * r_lse.abs()).all()
+
+
+@pytest.mark.parametrize("n", [1, 5, 8, 12, 16, 40])
+@pytest.mark.parametrize("d,dtype,e4m3,up", [(128, BF16, False, 60), (64, BF16, False, 30), (96, BF16, True, 60), (128, BF16, True, 27),
+                                             (64, F16, False, 27), (128, F16, True, 27), (128, BF16, False, 22), (64, BF16, True, 22)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_whose_rounding_is_larger_than_an_exponent(n, d, dtype, e4m3, up, sign):
+    """Finite scores of 2^up and more, over several tiles to a block: every row is its largest key's value, wherever the
+    second largest score is further below than the rounding of both."""
+    c = Cache([2500, 700, 5000], 8, d, 64, dtype, e4m3, seed=n)
+    q, scale = _q(3, n, 32, d, dtype, n), sign * 2.0 ** up
+    got = _attend(q, c, c.seqused_k, softmax_scale=scale)
+    check_attention(got, q, c, scale, True)
+    clear = 0
+    for z in range(3):
+        k, v = (x[z].repeat_interleave(4, 1).permute(1, 0, 2) for x in (c.k, c.v))
+        s = scale * q[z].double().permute(1, 0, 2) @ k.transpose(1, 2)
+        i, j = torch.arange(n, device="cuda")[:, None], torch.arange(c.lens[z], device="cuda")[None, :]
+        s = torch.where(j <= c.lens[z] - n + i, s, -torch.inf)
+        top, where = s.topk(2, -1)
+        size = abs(scale) * q[z].double().permute(1, 0, 2).abs() @ k.abs().transpose(1, 2)
+        # each score is off by e; one that is 40 below the largest has a weight of 2^-57
+        e = 2.0 ** -23 * ((d + 4) * size.amax(-1) + 8)
+        alone = top[..., 0] - top[..., 1] > 2 * e + 40
+        want = torch.gather(v, 1, where[..., :1].expand(-1, -1, d))
+        off = (got[0][z].double().permute(1, 0, 2) - want).abs()
+        assert (off <= UNIT[dtype] * 1.01 * want.abs() + 2.0 ** -24)[alone].all()
+        clear += int(alone.sum())
+    assert clear > 3 * n * 32 // 2
