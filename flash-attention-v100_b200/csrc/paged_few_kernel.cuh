@@ -101,6 +101,13 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) {
   asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"((unsigned short)v) : "memory");
 }
 
+// 2^(byte - 127 + e), byte a scale (255 is NaN) and e the exponent of queries: the sum of the two is ordinary where each alone need
+// not be.  (At 2^-126 scores are nothing, at 2^126 they are beyond fp32: beyond these it stays what it is.)
+__device__ __forceinline__ float scale_power(uint32_t byte, int e) {
+  const int sum = max(1, min(253, (int)byte + e));
+  return __uint_as_float(byte == 255 ? 0x7fc00000u : (uint32_t)sum << 23);
+}
+
 // Sums over the 32 lanes of N values each; lane l ends up with the total of value (l * N / 32) (N <= 32: of lanes
 // that share a value, each has it).  Every step exchanges half of the values that a lane still has.
 template <int N>
@@ -151,7 +158,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   __shared__ uint8_t code_select[kE4m3 ? T::kCodeStages : 1][32];    // which byte of it, two bits for each of four rows
   __shared__ uint8_t k_scale[kE4m3 ? 4 : 1][128];
   __shared__ __align__(8) uint8_t v_bf16[kE4m3 ? kStages : 1][8];
-  __shared__ float q_scale[4];
+  __shared__ int q_exponent[4];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_word;
   __shared__ int skip_cta;
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           sts128(q_smem + b * T::kQBytes + (c >> 3) * T::kQBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), pack_half2(f[0], f[1]),
                  pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
         }
-        if (lane == 0) q_scale[used & 3] = __uint_as_float(e < -126 ? 1u << (149 + e) : (uint32_t)(127 + e) << 23);
+        if (lane == 0) q_exponent[used & 3] = e;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_q_full[b]));
@@ -508,10 +515,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         rolled_wait(smem_u32(&bar_s_full[b]), (n >> 1) & 1, &abort_word, 11);
         tc_fence_after();
         float c = p.negate ? -p.scale_log2 : p.scale_log2;
-        if constexpr (kE4m3) {
-          if (kBf16) c *= q_scale[piece & 3];
-          c *= scale_value(k_scale[n & 3][tid]);
-        }
+        if constexpr (kE4m3) c *= scale_power(k_scale[n & 3][tid], kBf16 ? q_exponent[piece & 3] : 0);
         // The exponentials' arguments: with 16 rows they stay in registers between the vote and the exponentials, with more
         // they are formed twice.
         float x[16];

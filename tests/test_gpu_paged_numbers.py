@@ -82,3 +82,19 @@ def test_scores_whose_rounding_is_larger_than_an_exponent(n, d, dtype, e4m3, up,
         assert (off <= UNIT[dtype] * 1.01 * want.abs() + 2.0 ** -24)[alone].all()
         clear += int(alone.sum())
     assert clear > 3 * n * 32 // 2
+
+
+@pytest.mark.parametrize("n", [1, 6, 9, 16, 40])
+@pytest.mark.parametrize("up", [-122, -60, 60, 110])
+def test_tiny_queries_of_huge_keys(n, up):
+    """Queries of 2^up and keys of 2^-up (8 bits): ordinary scores, whose two factors are beyond, or below, normal numbers."""
+    from flash_attn_v100 import paged_cache_read, paged_cache_write
+
+    d, lens = 64, [300, 140]
+    c = Cache([0, 0], 2, d, 32, BF16, True, room=300)
+    k, v = (_q(2, 300, 2, d, BF16, i, 1.0) for i in (2, 3))
+    k = torch.ldexp(k.double(), torch.tensor(-up, device="cuda")).to(BF16)
+    paged_cache_write(k, v, *c.args(), _i32([0, 0]), **c.scales())
+    held = Held(*paged_cache_read(*c.args(), _i32(lens), 300, dtype=BF16, **c.scales()), lens, True)
+    q = torch.ldexp(_q(2, n, 8, d, BF16, 4).double(), torch.tensor(up, device="cuda")).to(BF16)
+    check_attention(_attend(q, c, _i32(lens)), q, held, d ** -0.5, True)
