@@ -140,7 +140,10 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   extern __shared__ uint8_t smem_raw[];
   __shared__ PagedPiece items[T::kItemStages];
   __shared__ uint64_t bar_item_full[T::kItemStages], bar_item_empty[T::kItemStages];
-  __shared__ uint64_t bar_kv_full[kStages], bar_kv_empty[kStages];
+  // bar_kv_empty: of a slot.  bar_k_full, bar_v_full: K, V of tile n have landed, n modulo kStages.  Not of a slot: with an odd
+  // number of slots one holds K and V by turns, each of which another warp waits for.  The issuer of S^T would come to wait for K(n)
+  // in a slot before V(n - 3) had landed there, and the parity it waits for would be that of the phase before.
+  __shared__ uint64_t bar_k_full[kE4m3 ? 1 : kStages], bar_v_full[kStages], bar_kv_empty[kStages];
   __shared__ uint64_t bar_q_full[2], bar_q_free[2], bar_s_full[2], bar_s_free[2], bar_p_full[2], bar_p_free[2],
       bar_o_full[2], bar_o_free[2];
   __shared__ float warp_part[4][kRows];   // per warp: a row's maximum, or its sum
@@ -186,7 +189,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       mbar_init(smem_u32(&bar_item_empty[s]), kE4m3 ? 11 + T::kVWarps : 7);  // two MMA, Q, four softmax (eight converting) warps
     }
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&bar_kv_full[s]), kE4m3 ? T::kVWarps : 1);
+      if (!kE4m3) mbar_init(smem_u32(&bar_k_full[s]), 1);
+      mbar_init(smem_u32(&bar_v_full[s]), kE4m3 ? T::kVWarps : 1);
       mbar_init(smem_u32(&bar_kv_empty[s]), 1);
     }
     for (int s = 0; s < T::kCodeStages; ++s) {
@@ -271,10 +275,10 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     const bool mine = sub < pages.parts();
     const uint32_t dst = (kE4m3 ? code_smem : ring_smem) + box * T::kBoxBytes + sub * p.box_rows * 128;
     const CUtensorMap* const tm = is_v ? &tm_v : &tm_k;
-    uint64_t* const fulls = kE4m3 ? bar_code_full : bar_kv_full;
+    uint64_t* const fulls = kE4m3 ? bar_code_full : is_v ? bar_v_full : bar_k_full;
     uint64_t* const empties = kE4m3 ? bar_code_empty : bar_kv_empty;
     bool ok = true;
-    uint32_t slot = 0, phase = 1, published = 0;
+    uint32_t slot = 0, phase = 1, published = 0, tile = 0;  // tile: modulo kStages
     auto next_item = [&]() -> PagedPiece {
       const PagedPiece it = published == 0 ? first_piece : work.next(p, blockIdx.x);
       const uint32_t s = published % T::kItemStages, round = published / T::kItemStages;
@@ -306,13 +310,14 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         ok = ok && rolled_wait_warp(smem_u32(&empties[slot]), phase, &abort_word, 3) &&
              rolled_wait_warp(smem_u32(&empties[slot_v]), phase_v, &abort_word, 4);
         if (!ok) break;
-        const uint32_t to = is_v ? slot_v : slot, full = smem_u32(&fulls[to]);
+        const uint32_t to = is_v ? slot_v : slot, full = smem_u32(&fulls[kE4m3 ? to : tile]);
         if ((lane & 15) == 0) mbar_arrive_expect_tx(full, kBytes);
         __syncwarp();
         if (mine) tma_load_4d(dst + to * kBytes, tm, full, box * 64, row, it.h, page);
         __syncwarp();
         phase = slot + 2 >= kRing ? phase ^ 1 : phase;
         slot = slot + 2 >= kRing ? slot + 2 - kRing : slot + 2;
+        tile = tile + 1 == (uint32_t)kStages ? 0 : tile + 1;
       }
       it = after;
       first_pages = first_pages_after;
@@ -387,7 +392,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   } else if (warp == 4) {
     // =========================== MMA issuer of S^T = K Q^T ===================
     // Each product has a warp of its own: issuing, the commits most of all, takes longer than the products themselves.
-    uint32_t n = 0, piece = 0, slot = 0, phase = 0;
+    uint32_t n = 0, piece = 0, slot = 0, tile = 0, phase = 0;  // tile: n modulo kStages, and the parity of its round
     bool ok = true;
     while (ok) {
       const PagedPiece it = take_item();
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         if (kE4m3)
           ok = ok && rolled_wait_warp(smem_u32(&bar_kt_full[b]), (n >> 1) & 1, &abort_word, 18);
         else
-          ok = ok && rolled_wait_warp(smem_u32(&bar_kv_full[slot]), phase, &abort_word, 9);
+          ok = ok && rolled_wait_warp(smem_u32(&bar_k_full[tile]), phase, &abort_word, 9);
         if (ok && n >= 2) ok = rolled_wait_warp(smem_u32(&bar_s_free[b]), ((n >> 1) - 1) & 1, &abort_word, 10);
         if (!ok) break;
         tc_fence_after();
@@ -420,8 +425,9 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           if (j == it.tiles - 1) umma_commit(smem_u32(&bar_q_free[qb]));
         }
         __syncwarp();
-        if ((slot += 2) >= (uint32_t)kStages) {
-          slot -= kStages;
+        if ((slot += 2) >= (uint32_t)kStages) slot -= kStages;
+        if (++tile == (uint32_t)kStages) {
+          tile = 0;
           phase ^= 1;
         }
       }
@@ -429,7 +435,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
     }
   } else if (warp == 7) {
     // =========================== MMA issuer of O^T += V^T P^T ===================
-    uint32_t n = 0, piece = 0, slot = kE4m3 ? 0 : 1, phase = 0;
+    uint32_t n = 0, piece = 0, slot = kE4m3 ? 0 : 1, tile = 0, phase = 0;
     bool ok = true;
     while (ok) {
       const PagedPiece it = take_item();
@@ -439,7 +445,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       for (int j = 0; j < it.tiles; ++j, ++n) {
         const uint32_t b = n & 1;
         if (j == 0 && piece >= 2) ok = rolled_wait_warp(smem_u32(&bar_o_free[ob]), ((piece >> 1) - 1) & 1, &abort_word, 7);
-        ok = ok && rolled_wait_warp(smem_u32(&bar_kv_full[slot]), phase, &abort_word, 6) &&
+        ok = ok && rolled_wait_warp(smem_u32(&bar_v_full[tile]), phase, &abort_word, 6) &&
              rolled_wait_warp(smem_u32(&bar_p_full[b]), (n >> 1) & 1, &abort_word, 5);
         if (!ok) break;
         tc_fence_after();
@@ -464,8 +470,9 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           if (j == it.tiles - 1) umma_commit(smem_u32(&bar_o_full[ob]));
         }
         __syncwarp();
-        if ((slot += kE4m3 ? 1 : 2) >= (uint32_t)kStages) {
-          slot -= kStages;
+        if ((slot += kE4m3 ? 1 : 2) >= (uint32_t)kStages) slot -= kStages;
+        if (++tile == (uint32_t)kStages) {
+          tile = 0;
           phase ^= 1;
         }
       }
@@ -605,8 +612,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         }
         if (!kE4m3 && key0 + 128 > it.sk) {
           // rows of V behind the entry's end
-          const uint32_t at = v_at(n), slot = at % kStages;
-          rolled_wait(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 13);
+          const uint32_t slot = v_at(n) % kStages;
+          rolled_wait(smem_u32(&bar_v_full[n % kStages]), n / kStages & 1, &abort_word, 13);
           if (key >= it.sk) {
 #pragma unroll
             for (int box = 0; box < T::kBoxes; ++box)
@@ -617,8 +624,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         }
         [[maybe_unused]] bool bf = false;
         if constexpr (kE4m3 && kBf16) {
-          const uint32_t at = v_at(n), slot = at % kStages;
-          rolled_wait(smem_u32(&bar_kv_full[slot]), at / kStages & 1, &abort_word, 17);
+          const uint32_t slot = n % kStages;
+          rolled_wait(smem_u32(&bar_v_full[slot]), n / kStages & 1, &abort_word, 17);
           bf = v_bf16[slot][tid >> 4] != 0;
         }
         if (n >= 2) rolled_wait(smem_u32(&bar_p_free[b]), ((n >> 1) - 1) & 1, &abort_word, 14);
@@ -812,7 +819,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(smem_u32(&bar_kv_full[slot]));
+            mbar_arrive(smem_u32(&bar_v_full[slot]));
             mbar_arrive(smem_u32(&bar_code_empty[from]));
           }
         }
