@@ -154,14 +154,15 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
   __shared__ long long row_out[kRows];              // where a row of O lies, from its block's first row on
   // 8-bit caches: codes and scale bytes of a stage; K in tensor memory, and its scale bytes (a tile's are read after the
   // next two may have been converted); whether 16 rows of V in a slot are bf16; the power of two that a piece's Q was divided
-  // by (Q is three pieces ahead at most)
+  // by (Q is three pieces ahead at most), or each row's where they are too unequal for one
   __shared__ uint64_t bar_code_full[kE4m3 ? T::kCodeStages : 1], bar_code_empty[kE4m3 ? T::kCodeStages : 1];
   __shared__ uint64_t bar_kt_full[2], bar_kt_free[2];
   __shared__ __align__(16) uint32_t code_scale[kE4m3 ? T::kCodeStages : 1][128];  // the aligned word around a row's byte
   __shared__ uint8_t code_select[kE4m3 ? T::kCodeStages : 1][32];    // which byte of it, two bits for each of four rows
   __shared__ uint8_t k_scale[kE4m3 ? 4 : 1][128];
   __shared__ __align__(8) uint8_t v_bf16[kE4m3 ? kStages : 1][8];
-  __shared__ int q_exponent[4];
+  constexpr int kUnequal = 1 << 20;  // in place of an exponent
+  __shared__ int q_exponent[4], q_row_exponent[kE4m3 && kBf16 ? 4 : 1][kRows];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_word;
   __shared__ int skip_cta;
@@ -337,8 +338,10 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
       if (round > 0 && !rolled_wait_warp(smem_u32(&bar_q_free[b]), (round - 1) & 1, &abort_word, 24)) break;
       if constexpr (kE4m3 && kBf16) {
         // Q in fp16, like K: divided by the power of two that brings its largest value to [2^14, 2^15).  What is less
-        // than 2^-28 of that value loses bits, nothing is off by more than 2^-39 of it.  Rows behind the entry's new tokens may
-        // hold anything: they have no say in it, and become zeros.
+        // than 2^-28 of that value loses bits, nothing is off by more than 2^-39 of it.  So rows whose largest values are within
+        // 2^13 of one another share one power (off by 2^-26 of a row's own at most, less than an fp32 sum is); others have one
+        // each, which the softmax multiplies their scores by.  Rows behind the entry's new tokens may hold anything: they have
+        // no say in it, and become zeros.
         const int total = p.seqlen_q * p.group * (DR / 8);  // chunks of 8 elements
         const int real = min(p.seqlen_q, it.sq - it.token0) * p.group * (DR / 8);
         const uint16_t* src = p.q + it.z * p.q_batch + it.token0 * p.q_row + it.h * p.group * p.q_head;
@@ -346,28 +349,51 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           const int r = n / (DR / 8), t = row_token(p, r);
           return __ldg(reinterpret_cast<const uint4*>(src + t * p.q_row + (r - t * p.group) * p.q_head) + n % (DR / 8));
         };
-        uint32_t top = 0;  // exponent fields of finite values
-#pragma unroll 1
-        for (int n = lane; n < real; n += 32) {
-          const uint4 x = chunk_of(n);
+        auto top_of = [](const uint4& x) {  // largest exponent field of a finite value
+          uint32_t top = 0;
           for (uint32_t w : {x.x, x.y, x.z, x.w})
             for (uint32_t ex : {w >> 7 & 0xffu, w >> 23 & 0xffu}) top = ex == 255 ? top : max(top, ex);
+          return top;
+        };
+        uint32_t most = 0, least = 255;
+#pragma unroll 1
+        for (int n = lane; n < real; n += 32) {
+          const uint32_t top = top_of(chunk_of(n));
+          most = max(most, top);
+          least = top == 0 ? least : min(least, top);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        const int e = top == 0 ? 0 : (int)top - 127 - 14;  // (-140 to 113)
-        // 2^-e in two factors: one alone need not be a normal number
-        const float s0 = __uint_as_float((uint32_t)(127 - e / 2) << 23), s1 = __uint_as_float((uint32_t)(127 - (e - e / 2)) << 23);
+        most = __reduce_max_sync(0xffffffffu, most);
+        least = __reduce_min_sync(0xffffffffu, least);
+        const int e = most == 0 ? 0 : (int)most - 127 - 14;  // (-140 to 113)
+        // (chunks within 2^13 of one another are of rows that are; where they are not, the rows may be)
+        bool unequal = most > least + 13;
+        int* const exponents = q_row_exponent[used & 3];
+        if (unequal) {
+          least = 255;
+          for (int r = lane; r < kRows; r += 32) exponents[r] = e;
+          __syncwarp();
+#pragma unroll 1
+          for (int n = 0; n < real; n += DR / 8) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, lane < DR / 8 ? top_of(chunk_of(n + lane)) : 0u);
+            least = top == 0 ? least : min(least, top);
+            if (lane == 0 && top != 0) exponents[n / (DR / 8)] = (int)top - 127 - 14;
+          }
+          unequal = most > least + 13;
+          __syncwarp();
+        }
 #pragma unroll 1
         for (int n = lane; n < total; n += 32) {
           float f[8];
           unpack8<__nv_bfloat16>(n < real ? chunk_of(n) : make_uint4(0, 0, 0, 0), f);
-          const int r = n / (DR / 8), c = n % (DR / 8);
+          const int r = n / (DR / 8), c = n % (DR / 8), er = unequal ? exponents[r] : e;
+          // 2^-er in two factors: one alone need not be a normal number
+          const float s0 = __uint_as_float((uint32_t)(127 - er / 2) << 23), s1 = __uint_as_float((uint32_t)(127 - (er - er / 2)) << 23);
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] = f[i] * s0 * s1;
           sts128(q_smem + b * T::kQBytes + (c >> 3) * T::kQBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), pack_half2(f[0], f[1]),
                  pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
         }
-        if (lane == 0) q_exponent[used & 3] = e;
+        if (lane == 0) q_exponent[used & 3] = unequal ? kUnequal : e;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_q_full[b]));
@@ -522,7 +548,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         rolled_wait(smem_u32(&bar_s_full[b]), (n >> 1) & 1, &abort_word, 11);
         tc_fence_after();
         float c = p.negate ? -p.scale_log2 : p.scale_log2;
-        if constexpr (kE4m3) c *= scale_power(k_scale[n & 3][tid], kBf16 ? q_exponent[piece & 3] : 0);
+        [[maybe_unused]] const int eq = kE4m3 && kBf16 ? q_exponent[piece & 3] : 0;
+        if constexpr (kE4m3) c *= scale_power(k_scale[n & 3][tid], eq);
         // The exponentials' arguments: with 16 rows they stay in registers between the vote and the exponentials, with more
         // they are formed twice.
         float x[16];
@@ -559,7 +586,20 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
         if (force) {
           // A new reference for every row: its largest score so far.  It is a rounded product, so this tile's scores become
           // rounded products, too, before it is taken off: in one step, a score of 2^28 could come out at 2^4 over itself, or
-          // under.  Where a reference exceeds 2^20, every tile takes new ones.
+          // under.  Where a reference exceeds 2^20, every tile takes new ones; and where rows have a power of two each, which a
+          // score of theirs is multiplied by here.
+          if constexpr (kE4m3 && kBf16) {
+            if (eq == kUnequal) {
+              const float base = p.negate ? -p.scale_log2 : p.scale_log2;
+              c = 1.f;
+#pragma unroll 1
+              for (int r = 0; r < kRows; ++r) {
+                const float s = tmem_ld1(tS + r);
+                tmem_st1(tS + r, s * (base * scale_power(k_scale[n & 3][tid], q_row_exponent[piece & 3][r])));
+              }
+              tmem_wait_st();
+            }
+          }
 #pragma unroll 1
           for (int r0 = 0; r0 < kRows; r0 += 16) {
             uint32_t s[16];
@@ -589,7 +629,7 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             ref = m;
             unset = m == -CUDART_INF_F ? row_last[tid] > key0 + 127 : fabsf(m) > 1048576.f;
           }
-          force = vote_any(1, 128, unset);
+          force = vote_any(1, 128, unset || (kE4m3 && kBf16 && eq == kUnequal));
           if (j > 0) {
             // O^T of the tiles before is complete
             rolled_wait(smem_u32(&bar_p_free[b ^ 1]), ((n - 1) >> 1) & 1, &abort_word, 12);

@@ -98,3 +98,20 @@ def test_tiny_queries_of_huge_keys(n, up):
     held = Held(*paged_cache_read(*c.args(), _i32(lens), 300, dtype=BF16, **c.scales()), lens, True)
     q = torch.ldexp(_q(2, n, 8, d, BF16, 4).double(), torch.tensor(up, device="cuda")).to(BF16)
     check_attention(_attend(q, c, _i32(lens)), q, held, d ** -0.5, True)
+
+
+@pytest.mark.parametrize("n", [1, 2, 5, 8, 11, 16, 40])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("up", [12, 30, 60, 100])
+def test_queries_of_very_unequal_size(n, d, e4m3, up):
+    """Heads and tokens of one item: ordinary ones, zeros, 2^up and 2^-up times the ordinary (bf16), over several tiles to a
+    block.  None of them is less exact for its neighbours."""
+    c = Cache([2500, 700, 5000], 8, d, 32, BF16, e4m3, seed=n)
+    q = _q(3, n, 32, d, BF16, n)
+    size = torch.ones((3, n, 32, 1), device="cuda")
+    size[:, :, 1::4] = 2.0 ** up
+    size[1, :, 2::4] = 2.0 ** -up
+    size[2, n // 2:, 3::4] = 0.0
+    q = (q.float() * size).to(BF16)
+    check_attention(_attend(q, c, c.seqused_k), q, c, d ** -0.5, True)
