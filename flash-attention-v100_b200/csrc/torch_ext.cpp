@@ -533,8 +533,7 @@ std::tuple<at::Tensor, at::Tensor> op_paged_fwd(const at::Tensor& q, const at::T
 
 // The cache serves; none of its functions has a derivative, and what autograd would have to know is refused
 // instead of dropped.
-void check_no_derivative(std::initializer_list<const at::Tensor*> inputs, const char* name) {
-  if (const auto& functorch = at::functorch::functorchTLSAccessor()) functorch->checkSupportsCppAutogradFunction();
+void check_no_gradient(std::initializer_list<const at::Tensor*> inputs, const char* name) {
   for (const at::Tensor* t : inputs) {
     TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()), name,
                 " has no derivative: call it under torch.no_grad(), or on inputs that require none");
@@ -542,6 +541,41 @@ void check_no_derivative(std::initializer_list<const at::Tensor*> inputs, const 
       TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), name,
                                   " has no forward-mode derivative (an input carries a tangent)");
   }
+}
+void check_no_derivative(std::initializer_list<const at::Tensor*> inputs, const char* name) {
+  if (const auto& functorch = at::functorch::functorchTLSAccessor()) functorch->checkSupportsCppAutogradFunction();
+  check_no_gradient(inputs, name);
+}
+
+// the dispatcher's entries
+const auto& paged_fwd_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("flash_attn_v100::paged_fwd", "")
+                             .typed<decltype(op_paged_fwd)>();
+  return op;
+}
+const auto& paged_write_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("flash_attn_v100::paged_write", "")
+                             .typed<decltype(op_paged_write)>();
+  return op;
+}
+const auto& paged_read_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("flash_attn_v100::paged_read", "")
+                             .typed<decltype(op_paged_read)>();
+  return op;
+}
+
+// what autograd saved of tensors that are written is no longer what they hold (tensors made under inference_mode keep no count)
+void count_versions(const at::Tensor& k_cache, const at::Tensor& v_cache, const OptTensor& k_scale, const OptTensor& v_scale) {
+  auto written = [](const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  written(k_cache);
+  written(v_cache);
+  if (k_scale.has_value()) written(*k_scale);
+  if (v_scale.has_value()) written(*v_scale);
 }
 
 // flash_attn_paged_func, paged_cache_write and paged_cache_read outside of tracing
@@ -552,35 +586,21 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at
                                                    std::optional<double> softmax_scale, bool causal) {
   TORCH_CHECK(q.dim() > 0, "q must have shape (batch, seqlen, heads, head_size)");
   check_no_derivative({&q, &k_cache, &v_cache}, "flash_attn_paged_func");
-  static const auto op = c10::Dispatcher::singleton()
-                             .findSchemaOrThrow("flash_attn_v100::paged_fwd", "")
-                             .typed<decltype(op_paged_fwd)>();
   at::AutoDispatchBelowADInplaceOrView guard;
-  return op.call(last_dim_contiguous(q), k_cache, v_cache, block_table, seqused_k, seqused_q, k_scale, v_scale,
-                 softmax_scale.has_value() ? *softmax_scale : std::pow((double)q.size(-1), -0.5), causal);
+  return paged_fwd_op().call(last_dim_contiguous(q), k_cache, v_cache, block_table, seqused_k, seqused_q, k_scale, v_scale,
+                             softmax_scale.has_value() ? *softmax_scale : std::pow((double)q.size(-1), -0.5), causal);
 }
 
 void paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
                  const at::Tensor& block_table, const at::Tensor& cache_seqlens, const OptTensor& seqused,
                  const OptTensor& k_scale, const OptTensor& v_scale) {
   check_no_derivative({&k, &v, &k_cache, &v_cache}, "paged_cache_write");
-  static const auto op = c10::Dispatcher::singleton()
-                             .findSchemaOrThrow("flash_attn_v100::paged_write", "")
-                             .typed<decltype(op_paged_write)>();
   {
     at::AutoDispatchBelowADInplaceOrView guard;
-    op.call(last_dim_contiguous(k), last_dim_contiguous(v), k_cache, v_cache, block_table, cache_seqlens, seqused,
-            k_scale, v_scale);
+    paged_write_op().call(last_dim_contiguous(k), last_dim_contiguous(v), k_cache, v_cache, block_table, cache_seqlens,
+                          seqused, k_scale, v_scale);
   }
-  // what autograd saved of these tensors before is no longer what they hold
-  // (tensors made under inference_mode keep no count)
-  auto written = [](const at::Tensor& t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  };
-  written(k_cache);
-  written(v_cache);
-  if (k_scale.has_value()) written(*k_scale);
-  if (v_scale.has_value()) written(*v_scale);
+  count_versions(k_cache, v_cache, k_scale, v_scale);
 }
 
 std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -588,11 +608,44 @@ std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& k_cache, const a
                                               int64_t seqlen, const OptTensor& k_scale, const OptTensor& v_scale,
                                               at::ScalarType dtype) {
   check_no_derivative({&k_cache, &v_cache}, "paged_cache_read");
-  static const auto op = c10::Dispatcher::singleton()
-                             .findSchemaOrThrow("flash_attn_v100::paged_read", "")
-                             .typed<decltype(op_paged_read)>();
   at::AutoDispatchBelowADInplaceOrView guard;
-  return op.call(k_cache, v_cache, block_table, seqused_k, seqlen, k_scale, v_scale, dtype);
+  return paged_read_op().call(k_cache, v_cache, block_table, seqused_k, seqlen, k_scale, v_scale, dtype);
+}
+
+// The same for direct calls of the ops and for what torch.compile traced, which come by the dispatcher's keys: gradients are
+// refused where autograd would record them, versions are counted where in-place changes are.
+void autograd_paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                          const at::Tensor& block_table, const at::Tensor& cache_seqlens, const OptTensor& seqused,
+                          const OptTensor& k_scale, const OptTensor& v_scale) {
+  check_no_gradient({&k, &v, &k_cache, &v_cache}, "flash_attn_v100::paged_write");
+  at::AutoDispatchBelowAutograd guard;
+  paged_write_op().call(k, v, k_cache, v_cache, block_table, cache_seqlens, seqused, k_scale, v_scale);
+}
+std::tuple<at::Tensor, at::Tensor> autograd_paged_read(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                       const at::Tensor& block_table, const at::Tensor& seqused_k,
+                                                       int64_t seqlen, const OptTensor& k_scale, const OptTensor& v_scale,
+                                                       at::ScalarType dtype) {
+  check_no_gradient({&k_cache, &v_cache}, "flash_attn_v100::paged_read");
+  at::AutoDispatchBelowAutograd guard;
+  return paged_read_op().call(k_cache, v_cache, block_table, seqused_k, seqlen, k_scale, v_scale, dtype);
+}
+std::tuple<at::Tensor, at::Tensor> autograd_paged_fwd(const at::Tensor& q, const at::Tensor& k_cache,
+                                                      const at::Tensor& v_cache, const at::Tensor& block_table,
+                                                      const at::Tensor& seqused_k, const OptTensor& seqused_q,
+                                                      const OptTensor& k_scale, const OptTensor& v_scale,
+                                                      double softmax_scale, bool causal) {
+  check_no_gradient({&q, &k_cache, &v_cache}, "flash_attn_v100::paged_fwd");
+  at::AutoDispatchBelowAutograd guard;
+  return paged_fwd_op().call(q, k_cache, v_cache, block_table, seqused_k, seqused_q, k_scale, v_scale, softmax_scale, causal);
+}
+void counted_paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                         const at::Tensor& block_table, const at::Tensor& cache_seqlens, const OptTensor& seqused,
+                         const OptTensor& k_scale, const OptTensor& v_scale) {
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    paged_write_op().call(k, v, k_cache, v_cache, block_table, cache_seqlens, seqused, k_scale, v_scale);
+  }
+  count_versions(k_cache, v_cache, k_scale, v_scale);
 }
 
 }  // namespace
@@ -623,10 +676,11 @@ TORCH_LIBRARY_IMPL(flash_attn_v100, CUDA, m) {
 TORCH_LIBRARY_IMPL(flash_attn_v100, Autograd, m) {
   m.impl("fwd", torch::autograd::autogradNotImplementedFallback());
   m.impl("bwd", torch::autograd::autogradNotImplementedFallback());
-  m.impl("paged_write", torch::autograd::autogradNotImplementedFallback());
-  m.impl("paged_read", torch::autograd::autogradNotImplementedFallback());
-  m.impl("paged_fwd", torch::autograd::autogradNotImplementedFallback());
+  m.impl("paged_write", TORCH_FN(autograd_paged_write));
+  m.impl("paged_read", TORCH_FN(autograd_paged_read));
+  m.impl("paged_fwd", TORCH_FN(autograd_paged_fwd));
 }
+TORCH_LIBRARY_IMPL(flash_attn_v100, ADInplaceOrView, m) { m.impl("paged_write", TORCH_FN(counted_paged_write)); }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "B200 (sm_100a) fused multi-head attention";
