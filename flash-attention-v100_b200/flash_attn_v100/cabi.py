@@ -492,8 +492,30 @@ def merge_parts(o_parts, lse_parts, row_offsets, o_out, lse_out, stream=None):
     return o_out, lse_out
 
 
+def _require_pool(k_cache, v_cache, block_table, k_scale, v_scale):
+    """Two pools (num_pages, page_size, heads, head_dim) of one type, scales where that is float8_e4m3fn and only there."""
+    e4m3 = k_cache.dtype == torch.float8_e4m3fn
+    for t in (k_cache, v_cache):
+        if t.dim() != 4 or t.shape != k_cache.shape or t.dtype != k_cache.dtype or t.stride(-1) != 1 \
+                or t.dtype not in (torch.float16, torch.bfloat16, torch.float8_e4m3fn):
+            raise RuntimeError("k_cache and v_cache must be (num_pages, page_size, heads, head_dim), of one shape and type "
+                               "(fp16, bf16 or float8_e4m3fn), with a contiguous last dimension")
+    if (k_scale is None) == e4m3 or (v_scale is None) == e4m3:
+        raise RuntimeError("k_scale and v_scale belong to float8_e4m3fn caches, and only to them")
+    for t in (k_scale, v_scale):
+        if t is not None and (t.shape != k_cache.shape[:3] or t.dtype not in (torch.float8_e8m0fnu, torch.uint8)):
+            raise RuntimeError("k_scale and v_scale must be float8_e8m0fnu or uint8 (num_pages, page_size, heads)")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise RuntimeError("block_table must be int32 (batch, max_pages) with contiguous rows")
+    for t in (k_cache, v_cache, block_table, k_scale, v_scale):
+        if t is not None and (not t.is_cuda or t.device != k_cache.device):
+            raise RuntimeError("caches, scales and block_table must be on one CUDA device")
+
+
 def paged_cache(k_cache, v_cache, block_table, k_scale=None, v_scale=None) -> FmhaPagedCache:
-    """The C struct for pools (num_pages, page_size, heads, head_dim) and their block table."""
+    """The C struct for pools (num_pages, page_size, heads, head_dim) and their block table; it keeps the tensors it
+    names (in its attribute ``tensors``)."""
+    _require_pool(k_cache, v_cache, block_table, k_scale, v_scale)
     c = FmhaPagedCache()
     c.k, c.v, c.block_table = k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr()
     c.block_table_stride = block_table.stride(0)
@@ -503,7 +525,20 @@ def paged_cache(k_cache, v_cache, block_table, k_scale=None, v_scale=None) -> Fm
         c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
         c.k_scale_strides, c.v_scale_strides = _strides(k_scale), _strides(v_scale)
     c.num_pages, c.page_size, c.max_pages = k_cache.shape[0], k_cache.shape[1], block_table.shape[1]
+    c.tensors = (k_cache, v_cache, block_table, k_scale, v_scale)
     return c
+
+
+def _require_fit(cache: FmhaPagedCache, batch: int, heads: int, x: torch.Tensor):
+    """The pools behind the struct (where ``paged_cache`` made it) are of this batch, these heads, and x's row and type."""
+    tensors = getattr(cache, "tensors", None)
+    if tensors is None:
+        return
+    k_cache, _, block_table = tensors[:3]
+    if block_table.shape[0] != batch or k_cache.shape[2] != heads or k_cache.shape[3] != x.shape[3] or k_cache.device != x.device \
+            or k_cache.dtype not in (x.dtype, torch.float8_e4m3fn):
+        raise RuntimeError("the cache must have a block table row per batch entry, the given heads, and the head dimension, "
+                           "device and type (or float8_e4m3fn) of the other tensors")
 
 
 def paged_fwd(q, cache: FmhaPagedCache, heads_k: int, seqused_k, scale: float, causal: bool = False, seqused_q=None,
@@ -511,6 +546,11 @@ def paged_fwd(q, cache: FmhaPagedCache, heads_k: int, seqused_k, scale: float, c
     """O, LSE through ``fmha_paged_fwd``; outputs and workspace allocated with torch unless passed in."""
     _require_cuda_half(q, out)
     Z, N, H, D = q.shape
+    _require_fit(cache, Z, heads_k, q)
+    if out is not None and out.shape != q.shape:
+        raise RuntimeError("out must have the shape of q")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (Z, H, N) or not lse.is_contiguous()):
+        raise RuntimeError("lse must be contiguous fp32 (batch, query heads, new tokens)")
     out = torch.empty((Z, N, H, D), dtype=q.dtype, device=q.device) if out is None else out
     lse = torch.empty((Z, H, N), dtype=torch.float32, device=q.device) if lse is None else lse
     p = FmhaPagedFwdParams()
