@@ -948,7 +948,7 @@ const char* fmha_status_string(int status) {
     case FMHA_ERR_NULL_POINTER: return "a required pointer is NULL";
     case FMHA_ERR_BAD_HEAD_DIM: return "head_dim must be 64, 96 or 128";
     case FMHA_ERR_BAD_SHAPE: return "sizes must be positive and scale finite and non-zero";
-    case FMHA_ERR_BAD_STRIDE: return "strides must be positive multiples of 8 elements";
+    case FMHA_ERR_BAD_STRIDE: return "strides must be positive multiples of 16 bytes";
     case FMHA_ERR_BAD_ALIGNMENT: return "pointers must be 16-byte aligned";
     case FMHA_ERR_WORKSPACE: return "workspace missing or too small";
     case FMHA_ERR_TENSOR_MAP: return "cuTensorMapEncodeTiled rejected a tensor";

@@ -177,7 +177,8 @@ def paged_cache_write(k, v, k_cache, v_cache, block_table, cache_seqlens, sequse
     block_table: int32 (batch, max_pages); token t of entry z is row t % page_size of page
     block_table[z, t // page_size].  cache_seqlens: int32 (batch,), tokens an entry holds already; its new
     ones follow them.  seqused: int32 (batch,) or None, how many of the new tokens are real.  What goes beyond
-    an entry's pages, or to a page that the pool does not have, is dropped.
+    an entry's pages, or to a page that the pool does not have, is dropped.  Entries may share pages; tokens that they
+    write to one place in one call have to be the same.
     """
     if torch.compiler.is_compiling():
         torch.ops.flash_attn_v100.paged_write(_maybe_contiguous(k), _maybe_contiguous(v), k_cache, v_cache, block_table,
@@ -214,7 +215,8 @@ def flash_attn_paged_func(q, k_cache, v_cache, block_table, seqused_k, seqused_q
     the keys j <= seqused_k[z] - seqused_q[z] + i.  Returns (batch, new tokens, query heads, head_dim), zeros
     where a token sees nothing or is padding, with ``return_lse`` also the log-sum-exp (batch, query heads,
     new tokens) in fp32, -inf there.  Lengths and pages are read on the device: a captured call follows them.
-    Has no derivative.
+    q's padding may hold anything.  A value (V) that is not finite can make NaN of its element in new tokens of its entry
+    and head that are before it, too (0 times it is NaN).  Has no derivative.
     """
     if torch.compiler.is_compiling():
         scale = q.shape[-1] ** (-0.5) if softmax_scale is None else float(softmax_scale)

@@ -364,7 +364,7 @@ typedef struct {
   uint8_t* v_scale;
   const int32_t* block_table;   /* device, `batch` rows of max_pages entries */
   int64_t block_table_stride;   /* entries between its rows (>= max_pages) */
-  /* `batch` is the stride between pages; in elements, multiples of 16 bytes.  The scales' may be anything. */
+  /* `batch` is the stride between pages; in elements, positive multiples of 16 bytes.  The scales': any positive ones. */
   FmhaStrides k_strides, v_strides, k_scale_strides, v_scale_strides;
   int32_t num_pages, page_size, max_pages;
   int32_t format; /* FMHA_CACHE_* */
@@ -380,8 +380,9 @@ typedef struct {
   int32_t batch, heads, seqlen, head_dim, dtype;
 } FmhaCacheWriteParams;
 
-/* New tokens' K and V into their pages.  Tokens behind an entry's capacity are dropped; two tokens of a call at
- * one place leave either of them, row by row.  seqlen = 0 or batch = 0 does nothing. */
+/* New tokens' K and V into their pages.  Tokens behind an entry's capacity are dropped.  Two tokens of a call at one place
+ * (entries that share the page, or a page that stands twice in a row of the table) must be the same, else what is there
+ * afterwards is a mix of both, a scale of one and codes of the other among it.  seqlen = 0 or batch = 0 does nothing. */
 int fmha_cache_write(const FmhaCacheWriteParams* p, void* stream);
 
 typedef struct {
@@ -415,7 +416,9 @@ typedef struct {
 
 /* Attention of new tokens over the cache that holds their K and V (and whatever came before): O and LSE as
  * fmha_fwd has them.  Lengths are read on the device, so a captured call follows them.  Cached rows behind an
- * entry's last token may hold anything, NaN included.  Work is cut evenly over the SMs and what was cut is joined:
+ * entry's last token, and rows of q behind its new ones, may hold anything, NaN included.  A key that is not finite makes
+ * NaN of the rows that see it and of no others.  An element of V that is not finite makes NaN of that element of the rows that
+ * see it, and may of that element of new tokens before them (0 times it is NaN), never of other entries or heads.  Work is cut evenly over the SMs and what was cut is joined:
  * that takes `workspace` (device, 16-byte aligned, of fmha_paged_fwd_workspace_bytes(p) bytes, which depends on sizes
  * only; its contents mean nothing before or after, and calls that may overlap need one each; the size query is 0 where
  * fmha_paged_fwd refuses the sizes or has nothing to do).  FMHA_ERR_TOO_LARGE where seqlen_q * heads_q comes to 2^31,
