@@ -38,7 +38,7 @@
 // What bounds it.  16 bits, head dimension 128: HBM (32 entries of 2048 to 16384 keys, 32 query heads over 8: 182 us for 1.21
 // GB, 6.6 TB/s, the rate of a copy).  Otherwise a tile's way through the softmax warps: 1470 clk at head dimension 64, 16
 // bits, where 32 KB come in 1370 (16 entries of 16 heads: 4.3 TB/s), and 2200 to 2800 clk beside the converting warps, which
-// wait for it (64 entries in 8 bits: 309 us, 3.9 TB/s).  Short calls: 10 us of start, first loads, last tile and join.
+// wait for it (64 entries in 8 bits: 311 us, 3.9 TB/s).  Short calls: 10 us of start, first loads, last tile and join.
 // A second group of softmax warps, which takes every other tile, was tried twice and taken back: 16 bits no faster, 8 bits
 // 309 -> 359 (four warps for V) and 393 (eight; 80 registers a thread), only head dimension 64 in 8 bits gained (296 -> 270).
 #pragma once
@@ -355,8 +355,10 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             for (uint32_t ex : {w >> 7 & 0xffu, w >> 23 & 0xffu}) top = ex == 255 ? top : max(top, ex);
           return top;
         };
+        // (four loads at a time where there are more than a few: 40 rows, 49.3 -> 43.7 us a call; with 16 rows the code costs more than
+        // they take: 311 -> 319, 64 entries)
         uint32_t most = 0, least = 255;
-#pragma unroll 1
+#pragma unroll(kRows == 16 ? 1 : 4)
         for (int n = lane; n < real; n += 32) {
           const uint32_t top = top_of(chunk_of(n));
           most = max(most, top);
@@ -381,13 +383,15 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           unequal = most > least + 13;
           __syncwarp();
         }
+        // 2^-e in two factors: one alone need not be a normal number
+        auto factor = [](int half) { return __uint_as_float((uint32_t)(127 - half) << 23); };
+        float s0 = factor(e / 2), s1 = factor(e - e / 2);
 #pragma unroll 1
         for (int n = lane; n < total; n += 32) {
           float f[8];
           unpack8<__nv_bfloat16>(n < real ? chunk_of(n) : make_uint4(0, 0, 0, 0), f);
-          const int r = n / (DR / 8), c = n % (DR / 8), er = unequal ? exponents[r] : e;
-          // 2^-er in two factors: one alone need not be a normal number
-          const float s0 = __uint_as_float((uint32_t)(127 - er / 2) << 23), s1 = __uint_as_float((uint32_t)(127 - (er - er / 2)) << 23);
+          const int r = n / (DR / 8), c = n % (DR / 8);
+          if (unequal) s0 = factor(exponents[r] / 2), s1 = factor(exponents[r] - exponents[r] / 2);
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] = f[i] * s0 * s1;
           sts128(q_smem + b * T::kQBytes + (c >> 3) * T::kQBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), pack_half2(f[0], f[1]),

@@ -17,9 +17,9 @@
 //   warps 12-15     codes times scale -> the tensors' type, into the ring that 16-bit caches load directly
 //
 // What bounds it: the turns of tensor pipe and softmax, as in fwd_kernel.cuh.  2048 tokens over 16384 keys, 32 query heads over 8,
-// head dimension 128, bf16, causal: 605 to 617 us, 835 to 853 TFLOP/s (without a mask 931); keys of unequal size, as these
+// head dimension 128, bf16, causal: 560 to 617 us on different GPUs, 835 to 918 TFLOP/s; keys of unequal size, as these
 // were, make a new reference of the softmax more often than N(0, 1) does.  8-bit caches: the four converting warps take as long as a
-// round (six entries of 512 to 8192 keys, 1 to 512 new tokens each: 284 us, in 16 bits 208).
+// round (six entries of 1024 to 8192 keys, 1 to 512 new tokens each: 306 us, in 16 bits 219).
 #pragma once
 #include <cuda.h>
 

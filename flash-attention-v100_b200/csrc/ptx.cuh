@@ -84,7 +84,8 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity)
 // Bounded wait. `abort_word` is a word in shared memory shared by the whole CTA:
 // non-zero means some wait already ran out, and every wait then returns false at once.
 // The limit (about 2^22 polls, each a try_wait with the hardware's own short suspend)
-// is seconds of wall time, far above any legitimate wait in these kernels.
+// is far above any legitimate wait in these kernels: seconds of wall time where something wakes
+// the thread in between, minutes where nothing does (seen once: a wait for a tile that nobody loaded).
 constexpr uint32_t kWaitPollLimit = 1u << 22;
 
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_word,
