@@ -960,7 +960,7 @@ const char* fmha_status_string(int status) {
   }
 }
 
-const char* fmha_version(void) { return "0.4.0"; }
+const char* fmha_version(void) { return "0.4.1"; }
 
 #ifdef FMHA_TIMELINE
 // debug builds only: device buffer (>= 3 * 512 int64) and the CTA whose events are recorded

@@ -382,7 +382,8 @@ typedef struct {
 
 /* New tokens' K and V into their pages.  Tokens behind an entry's capacity are dropped.  Two tokens of a call at one place
  * (entries that share the page, or a page that stands twice in a row of the table) must be the same, else what is there
- * afterwards is a mix of both, a scale of one and codes of the other among it.  seqlen = 0 or batch = 0 does nothing. */
+ * afterwards is a mix of both, a scale of one and codes of the other among it.  seqlen = 0 or batch = 0 does nothing.
+ * FMHA_ERR_TOO_LARGE where seqlen * heads exceeds 2^27, or batch times that 2^34; so, too, in fmha_cache_read. */
 int fmha_cache_write(const FmhaCacheWriteParams* p, void* stream);
 
 typedef struct {
