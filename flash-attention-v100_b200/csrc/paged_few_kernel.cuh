@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
             for (uint32_t ex : {w >> 7 & 0xffu, w >> 23 & 0xffu}) top = ex == 255 ? top : max(top, ex);
           return top;
         };
-        // (four loads at a time where there are more than a few: 40 rows, 49.3 -> 43.7 us a call; with 16 rows the code costs more than
-        // they take: 311 -> 319, 64 entries)
+        // (Four loads at a time where there are more than a few: 40 rows, 49.3 -> 43.7 us a call.  With 16 rows the code costs
+        // more than they take: 64 entries 311 -> 319.)
         uint32_t most = 0, least = 255;
 #pragma unroll(kRows == 16 ? 1 : 4)
         for (int n = lane; n < real; n += 32) {
@@ -573,9 +573,9 @@ __global__ void __launch_bounds__(FewTraits<D, DR, kBf16, kE4m3, kRows>::kThread
           }
         };
         if (j > 0) {
-          // Would an exponential be too large?  (2^10 over the reference: P has to stay below the 65504 of fp16.)  Rows that see no key, padding
-          // among them, have no say: their arguments are -inf, or NaN, which the maximum passes over.  (A NaN of a row that
-          // does see the key makes P and the row sum NaN whatever the reference is.)
+          // Would an exponential be too large?  (2^10 over the reference: P has to stay below the 65504 of fp16.)  Rows that see
+          // no key, padding among them, have no say: their arguments are -inf, or NaN, which the maximum passes over.  (A NaN of
+          // a row that does see the key makes P and the row sum NaN whatever the reference is.)
           float top = -CUDART_INF_F;
 #pragma unroll
           for (int r0 = 0; r0 < kRows; r0 += 16) {
