@@ -415,16 +415,16 @@ typedef struct {
   int32_t* status;
 } FmhaPagedFwdParams;
 
-/* Attention of new tokens over the cache that holds their K and V (and whatever came before): O and LSE as
- * fmha_fwd has them.  Lengths are read on the device, so a captured call follows them.  Cached rows behind an
- * entry's last token, and rows of q behind its new ones, may hold anything, NaN included.  A key that is not finite makes
- * NaN of the rows that see it and of no others.  An element of V that is not finite makes NaN of that element of the rows that
- * see it, and may of that element of new tokens before them (0 times it is NaN), never of other entries or heads.  Work is cut evenly over the SMs and what was cut is joined:
- * that takes `workspace` (device, 16-byte aligned, of fmha_paged_fwd_workspace_bytes(p) bytes, which depends on sizes
- * only; its contents mean nothing before or after, and calls that may overlap need one each; the size query is 0 where
- * fmha_paged_fwd refuses the sizes or has nothing to do).  FMHA_ERR_TOO_LARGE where seqlen_q * heads_q comes to 2^31,
- * batch * heads_q * (seqlen_q + 256) to 2^34, or batch * heads_k * blocks of new tokens * KV tiles of 128 that the block
- * table has room for to 2^31. */
+/* Attention of new tokens over the cache that holds their K and V (and whatever came before): O and LSE as fmha_fwd
+ * has them. Lengths are read on the device, so a captured call follows them. Cached rows behind an entry's last
+ * token, and rows of q behind its new ones, may hold anything, NaN included. A key that is not finite makes NaN of
+ * the rows that see it and of no others. An element of V that is not finite makes NaN of that element of the rows
+ * that see it, and may of that element of new tokens before them (0 times it is NaN), never of other entries or
+ * heads. Work is cut evenly over the SMs and what was cut is joined: that takes `workspace` (device, 16-byte aligned,
+ * of fmha_paged_fwd_workspace_bytes(p) bytes, which depends on sizes only; its contents mean nothing before or after,
+ * and calls that may overlap need one each; the size query is 0 where fmha_paged_fwd refuses the sizes or has nothing
+ * to do). FMHA_ERR_TOO_LARGE where seqlen_q * heads_q comes to 2^31, batch * heads_q * (seqlen_q + 256) to 2^34, or
+ * batch * heads_k * blocks of new tokens * KV tiles of 128 that the block table has room for to 2^31. */
 size_t fmha_paged_fwd_workspace_bytes(const FmhaPagedFwdParams* p);
 int fmha_paged_fwd(const FmhaPagedFwdParams* p, void* workspace, size_t workspace_bytes, void* stream);
 
